@@ -43,6 +43,7 @@ _lib = None
 MISSING: list = []   # declared in ctamd.h but absent from the built library (tests assert it is empty)
 
 _vp, _i, _sz, _d, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_double, C.c_float
+_i64 = C.c_int64
 _ip = C.POINTER(C.c_int)
 
 # name -> (restype, argtypes); must list every symbol of include/ctamd.h
@@ -111,6 +112,16 @@ SIGNATURES = {
     "ct_correction_legacy_workspace_bytes": (_sz, [_ip, _i]),
     "ct_accurate_correction_legacy": (_i, [_vp, _vp, _i, _ip, _i, _i, _d, _i, _vp, _vp, _vp, _ip, _vp, _vp, _vp, _vp, _i, _ip, _vp, _sz, _vp]),
     "ct_trim_mean": (_i, [_vp, _i, _i, _d, _vp, _vp]),
+    "ct_grouped_product_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "ct_grouped_product": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _i64, _f, _i, _vp, _i64, _vp, _sz, _vp]),
+    "ct_grouped_product_dw_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "ct_grouped_product_dw": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "ct_gradset_table_bytes": (_sz, [_i]),
+    "ct_gradset_workspace_bytes": (_sz, []),
+    "ct_gradset_chunks": (_i64, [_i, C.POINTER(_i64)]),
+    "ct_gradset_write": (_i, [_i, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_i64), _ip, _vp, _sz, _vp]),
+    "ct_gradset_norm": (_i, [_vp, _i, _i64, _vp, _vp, _sz, _vp]),
+    "ct_gradset_clip": (_i, [_vp, _i, _i64, _d, _vp, _vp, _sz, _vp]),
     "ct_segment_workspace_bytes": (_sz, [_ip, _i]),
     "ct_segment_centroids": (_i, [_vp, _ip, _f, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ct_watershed_workspace_bytes": (_sz, [_ip, _i]),

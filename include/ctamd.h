@@ -296,6 +296,50 @@ int ct_legacy_predict_pos_batched(ct_ffn_t* ffn, int B, const double* const* seg
 int ct_trim_mean(const double* stack, int k, int n3, double cut, double* out, ct_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Dense layers of ragged row groups, their gradients, and the gradient norm  (ffn.py:56-265)
+ * ------------------------------------------------------------------------------------------ */
+#define CT_F32   0           /* value types of the entry points below */
+#define CT_BF16  1
+#define CT_F16   2
+
+/* Rows r of x in offsets[g] <= r < offsets[g + 1] are multiplied with the weight block of group g (the FFN's second layer is the case G = 2:
+ * reference cells with W2[:512], target cells with W2[512:], ffn.py:258-265):
+ *     y[r][n] = act(scale[g][n] * sum_k x[r][k] w[g][k][n] + shift[g][n]),   act(v) = v >= 0 ? v : slope * v
+ * x [dev] `type` [rows][K], row stride ldx; w [dev] `type` [G][K][N], or [G][N][K] with w_transposed (then this is the product's gradient with
+ * respect to x: x = dy, K = the layer's width, N = its input's), row stride ldw, group stride w_group_stride (0: one block for all groups);
+ * y [dev] `out_type` (= type, or CT_F32) [rows][N], row stride ldy; the last index is contiguous everywhere, strides count values, any alignment of a value.
+ * offsets [dev] int32 [G + 1], rising from 0 (offsets that do not are clamped: no access outside the tensors, but rows without a defined value).
+ * scale, shift [dev] fp32 [G][N] with group stride affine_stride (0: one row for all groups), either may be NULL; slope 1: no activation.
+ * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap x or w.  Sums are 32-bit; fp32 products are exact
+ * multiply-adds in ascending order of k within each block of 16.  Workspace: ct_grouped_product_workspace_bytes (may be 0: then NULL is fine).
+ * CT_ESHAPE beyond 2^24 tiles.                                                                                                           */
+size_t ct_grouped_product_workspace_bytes(int type, int rows, int K, int N, int G);
+int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
+                       int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
+                       float slope, int fill_tail, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, ct_stream_t stream);
+
+/* The gradient of ct_grouped_product (without scale, shift, act) with respect to w:
+ *     dw[g][k][n] = sum over the rows r of group g of x[r][k] dy[r][n];   zero for a group without rows
+ * dw [dev] `out_type` [G][K][N], row stride lddw, group stride dw_group_stride (groups must not overlap).  The sum's order depends on the sizes alone. */
+size_t ct_grouped_product_dw_workspace_bytes(int type, int rows, int K, int N, int G);
+int ct_grouped_product_dw(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* dy, int64_t lddy, int N,
+                          const int32_t* offsets, int G, void* dw, int64_t dw_group_stride, int64_t lddw, void* workspace, size_t workspace_bytes,
+                          ct_stream_t stream);
+
+/* The l2 norm over a list of gradients, and the list scaled to at most clip_norm (Keras' global_clipnorm):
+ *     norm = sqrt(sum of all squares);   out_i = in_i * clip_norm / max(norm, clip_norm);   norm not finite: every value NaN
+ * ct_gradset_write puts the list (host arrays of n [dev] addresses, lengths, types CT_F32 / CT_BF16 / CT_F16; out NULL: in place) into `table`
+ * [dev], 8-byte aligned; a table serves any number of later calls while the tensors stay where they are.  chunks = ct_gradset_chunks(n, sizes).
+ * norm [dev] fp32 [1].  Squares are summed in 64 bits in an order that depends on the sizes alone.  out_i must be in_i itself or overlap nothing. */
+size_t  ct_gradset_table_bytes(int n);
+size_t  ct_gradset_workspace_bytes(void);
+int64_t ct_gradset_chunks(int n, const int64_t* sizes);
+int ct_gradset_write(int n, const void* const* in, void* const* out, const int64_t* sizes, const int* types, void* table, size_t table_bytes,
+                     ct_stream_t stream);
+int ct_gradset_norm(const void* table, int n, int64_t chunks, float* norm, void* workspace, size_t workspace_bytes, ct_stream_t stream);
+int ct_gradset_clip(const void* table, int n, int64_t chunks, double clip_norm, float* norm, void* workspace, size_t workspace_bytes, ct_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Pre-processing: local contrast normalisation  (preprocess.py:85-188)
  * ------------------------------------------------------------------------------------------
  * dtype: 0 = uint16, 1 = float32.  img/data [dev], [x][y][z].
