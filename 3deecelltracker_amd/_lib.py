@@ -114,8 +114,8 @@ SIGNATURES = {
     "ct_trim_mean": (_i, [_vp, _i, _i, _d, _vp, _vp]),
     "ct_grouped_product_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "ct_grouped_product": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _i64, _f, _i, _vp, _i64, _vp, _sz, _vp]),
-    "ct_grouped_product_dw_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
-    "ct_grouped_product_dw": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "ct_grouped_product_grad_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "ct_grouped_product_grad": (_i, [_i, _i, _vp, _i64, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i64, _vp, _sz, _vp]),
     "ct_gradset_table_bytes": (_sz, [_i]),
     "ct_gradset_workspace_bytes": (_sz, []),
     "ct_gradset_chunks": (_i64, [_i, C.POINTER(_i64)]),

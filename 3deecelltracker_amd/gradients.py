@@ -11,7 +11,7 @@ import ctypes as C
 import math
 
 from . import _dev, _lib
-from .grouped import _types
+from .grouped import _On, _env
 
 
 def _dense(a):
@@ -25,12 +25,11 @@ def _dense(a):
 
 
 def _checked(grads, out):
-    t = _lib.require_gpu()
+    t, kinds, _ = _env()
     grads = list(grads)
     out = grads if out is None else list(out)
     if len(out) != len(grads):
         raise ValueError(f"out: {len(out)} tensors for {len(grads)} gradients")
-    kinds = _types()
     device = None
     for i, (g, o) in enumerate(zip(grads, out)):
         for a in (g, o):
@@ -78,11 +77,10 @@ class GradientSet:
     def __init__(self, grads, out=None):
         self._init(grads, out)
         if self._device is not None:
-            t = _lib.require_gpu()
-            t.cuda.current_stream(self._device).synchronize()
+            _env()[0].cuda.current_stream(self._device).synchronize()
 
     def _init(self, grads, out, once=False):
-        t = _lib.require_gpu(); L = _lib.lib()
+        t, kinds, L = _env()
         self.grads, self.out, self._device = _checked(grads, out)
         self._n = len(self.grads)
         if self._device is None:                              # an empty list: its norm is zero, on the current device
@@ -91,23 +89,24 @@ class GradientSet:
             raise ValueError("GradientSet: make the set before the capture begins")
         n, m = self._n, max(self._n, 1)
         sizes = (C.c_int64 * m)(*[g.numel() for g in self.grads])
-        types = (C.c_int * m)(*[_types()[g.dtype] for g in self.grads])
+        types = (C.c_int * m)(*[kinds[g.dtype] for g in self.grads])
         ins = (C.c_void_p * m)(*[g.data_ptr() for g in self.grads])
         outs = (C.c_void_p * m)(*[o.data_ptr() for o in self.out])
         self._chunks = L.ct_gradset_chunks(n, sizes)
-        with t.cuda.device(self._device):
+        with _On(t, self._device) as stream:
             self._table = _dev.workspace(L.ct_gradset_table_bytes(n), self._device)
-            _lib.check(L.ct_gradset_write(n, ins, outs, sizes, types, self._table.data_ptr(), self._table.numel(), _dev.stream(self._device)),
-                       "ct_gradset_write")
+            _lib.check(L.ct_gradset_write(n, ins, outs, sizes, types, self._table.data_ptr(), self._table.numel(), stream), "ct_gradset_write")
+        self._ws = L.ct_gradset_workspace_bytes()
 
     def _call(self, name, *args):
-        t = _lib.require_gpu(); L = _lib.lib()
-        with t.cuda.device(self._device):
-            norm = _dev.empty((), t.float32, self._device)
-            ws = _dev.workspace(L.ct_gradset_workspace_bytes(), self._device)
-            _lib.check(getattr(L, name)(self._table.data_ptr(), self._n, self._chunks, *args, norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                                        _dev.stream(self._device)), name)
-        return norm
+        t, _, L = _env()
+        # the scalar and the partial sums, new for each call: two streams, or two graphs, share none
+        scalar, ws = t.empty((), dtype=t.float32, device=self._device), t.empty(self._ws, dtype=t.uint8, device=self._device)
+        with _On(t, self._device) as stream:
+            rc = getattr(L, name)(self._table.data_ptr(), self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws, stream)
+        if rc:
+            _lib.check(rc, name)
+        return scalar
 
     def norm(self):
         """The l2 norm over all values, a float32 scalar on the device (asynchronous)."""

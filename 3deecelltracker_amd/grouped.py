@@ -16,47 +16,52 @@ from typing import Sequence, Union
 from . import _dev, _lib
 
 MAX_GROUPS = 1 << 20
+_ready = None
 
 
-def _types():
-    t = _lib.require_gpu()
-    return {t.float32: 0, t.bfloat16: 1, t.float16: 2}          # CT_F32, CT_BF16, CT_F16
+def _env():
+    """(torch, {type: CT_F32 / CT_BF16 / CT_F16}, the library), looked up once: these calls are short enough for the look-ups to count"""
+    global _ready
+    if _ready is None:
+        t = _lib.require_gpu()
+        _ready = (t, {t.float32: 0, t.bfloat16: 1, t.float16: 2}, _lib.lib())
+    return _ready
 
 
-def _check_matrix(name, a, dims, dtype=None, device=None):
-    t = _lib.require_gpu()
+def _check_tensor(t, types, name, a, dims, dtype, device):
+    """What every operand has to be; dtype, device None: the first one"""
     if not isinstance(a, t.Tensor) or not a.is_cuda:
         raise ValueError(f"{name}: expected a tensor on the GPU")
     if a.dim() != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got the shape {tuple(a.shape)}")
-    if a.dtype not in _types():
-        raise ValueError(f"{name}: values of type {a.dtype} are not supported (float32, bfloat16, float16)")
-    if dtype is not None and a.dtype != dtype:
-        raise ValueError(f"{name}: values are {a.dtype}, expected {dtype}")
+    if a.dtype is not dtype:
+        if dtype is not None:
+            raise ValueError(f"{name}: values are {a.dtype}, expected {dtype}")
+        if a.dtype not in types:
+            raise ValueError(f"{name}: values of type {a.dtype} are not supported (float32, bfloat16, float16)")
     if device is not None and a.device != device:
         raise ValueError(f"{name}: is on {a.device}, the other tensors are on {device}")
     if a.requires_grad and t.is_grad_enabled():
         raise ValueError(f"{name}: requires grad, but this product is not part of torch's graph: pass {name}.detach() and use product_grad")
 
 
-def _row_stride(name, a):
-    """Stride of the rows of [..., rows, columns]; a single row or column may carry any stride."""
-    rows, cols = a.shape[-2], a.shape[-1]
-    if cols > 1 and a.stride(-1) != 1:
-        raise ValueError(f"{name}: the last index must be contiguous (strides {tuple(a.stride())})")
+def _row_stride(name, rows, cols, row_stride, col_stride):
+    """Stride of the rows of [rows, columns]; a single row or column may carry any stride."""
+    if cols > 1 and col_stride != 1:
+        raise ValueError(f"{name}: the last index must be contiguous, its stride is {col_stride}")
     if rows <= 1 or cols == 0:
-        return max(cols, 1)
-    if a.stride(-2) < cols:
-        raise ValueError(f"{name}: rows overlap (strides {tuple(a.stride())})")
-    return a.stride(-2)
+        return cols or 1
+    if row_stride < cols:
+        raise ValueError(f"{name}: rows overlap (stride {row_stride} for {cols} columns)")
+    return row_stride
 
 
 def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, rows: int, device):
     """int32 [groups + 1] on `device`.  Numbers on the host (a sequence, an array, a CPU tensor) are checked and uploaded; a tensor that is on
     the device already (a router's counts, summed there) is taken as it is, since looking at it would wait for the stream."""
-    t = _lib.require_gpu()
+    t = _env()[0]
     if isinstance(offsets, t.Tensor) and offsets.is_cuda:
-        if offsets.dtype != t.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
+        if offsets.dtype is not t.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
             raise ValueError(f"offsets: expected a contiguous int32 tensor of {groups + 1} numbers, got {offsets.dtype} {tuple(offsets.shape)}")
         if offsets.device != device:
             raise ValueError(f"offsets: are on {offsets.device}, the other tensors are on {device}")
@@ -70,37 +75,55 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
 
 
 def _affine(name, a, groups, n, device):
-    t = _lib.require_gpu()
-    if a is None:
-        return None
-    if not isinstance(a, t.Tensor) or not a.is_cuda or a.device != device or a.dtype != t.float32 or a.dim() not in (1, 2):
+    """[n] or [groups, n] -> (tensor with contiguous rows, stride of its groups)"""
+    t = _env()[0]
+    if not isinstance(a, t.Tensor) or not a.is_cuda or a.device != device or a.dtype is not t.float32 or a.dim() not in (1, 2):
         raise ValueError(f"{name}: expected a float32 tensor [{n}] or [{groups}, {n}] on {device}")
-    a = a.unsqueeze(0) if a.dim() == 1 else a
-    if a.shape[1] != n or a.shape[0] not in (1, groups):
+    if a.shape[-1] != n or (a.dim() == 2 and a.shape[0] not in (1, groups)):
         raise ValueError(f"{name}: shape {tuple(a.shape)} does not fit {groups} groups of {n} columns")
-    return a.expand(groups, n)
+    a = a.contiguous()
+    return a, n if a.dim() == 2 and a.shape[0] == groups and groups > 1 else 0
 
 
-def _groups(w):
-    """(transposed, row stride, group stride) of w [G][K][N]; a view with K contiguous is read transposed."""
+def _weights(name, w, transposed):
+    """w [G][K][N] ([G][N][K] if transposed) -> (G, K, N, read transposed, row stride, group stride); a block may be laid out either way"""
     g, k, n = w.shape
-    flip = n > 1 and w.stride(2) != 1 and k >= 1 and w.stride(1) == 1
-    ld = _row_stride("w", w.transpose(1, 2) if flip else w)
-    group = 0 if g == 1 else w.stride(0)
-    if group < 0:
-        raise ValueError("w: negative strides")
-    return flip, ld, group
+    sg, sk, sn = w.stride()
+    if transposed:
+        k, n, sk, sn = n, k, sn, sk
+    if g < 1 or g > MAX_GROUPS or n < 1 or k < 1:
+        raise ValueError(f"{name}: shape {tuple(w.shape)} is empty or has more than {MAX_GROUPS} groups")
+    flip = (sn != 1 and sk == 1 and n > 1) or (transposed and sk == 1 and not (sn == 1 and k > 1))
+    ld = _row_stride(name, n, k, sn, sk) if flip else _row_stride(name, k, n, sk, sn)
+    return g, k, n, flip, ld, 0 if g == 1 else sg
+
+
+def _span(a):
+    """The bytes from a tensor's first value to its last"""
+    p = a.data_ptr()
+    return p, p + (sum((s - 1) * st for s, st in zip(a.shape, a.stride())) + 1) * a.element_size() if a.numel() else p
 
 
 def _overlap(a, b):
-    """Whether the byte ranges that two tensors span meet."""
-    def span(x):
-        last = sum((s - 1) * st for s, st in zip(x.shape, x.stride()))
-        return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (p, q), (r, s) = span(a), span(b)
+    (p, q), (r, s) = _span(a), _span(b)
     return p < s and r < q
+
+
+class _On:
+    """The calls run on the calling thread's current device: make it the tensors' where it is another, and name its current stream"""
+
+    def __init__(self, t, device):
+        self._guard = t.cuda.device(device) if t.cuda.current_device() != device.index else None
+        self.stream = t._C._cuda_getCurrentRawStream(device.index)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *a):
+        if self._guard is not None:
+            self._guard.__exit__(*a)
 
 
 def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, slope: float = 1.0, out=None, out_dtype=None):
@@ -109,47 +132,44 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
     x [rows, K]; w [G, K, N] of the same type (transposed=True: [G, N, K]; w.expand(G, K, N) shares one block); offsets: G + 1 numbers, on
     the host or as int32 on the device; scale, shift: float32 [N] or [G, N].  Sums are held in 32 bits and rounded once to `out_dtype`
     (x's type, or float32).  Rows behind offsets[G] are zero in a new result and stay as they were in a given `out` [rows, N].  -> [rows, N]"""
-    t = _lib.require_gpu(); L = _lib.lib()
-    _check_matrix("x", x, 2)
-    _check_matrix("w", w, 3, x.dtype, x.device)
-    if transposed:
-        w = w.transpose(1, 2)
-    g, k, n = w.shape
-    rows = x.shape[0]
-    if x.shape[1] != k:
-        raise ValueError(f"x has {x.shape[1]} columns, the weight blocks have {k} rows")
-    if g < 1 or g > MAX_GROUPS or n < 1 or k < 1:
-        raise ValueError(f"w: shape {tuple(w.shape)} is empty or has more than {MAX_GROUPS} groups")
-    dtype = out.dtype if out is not None and out_dtype is None else out_dtype or x.dtype
-    if dtype not in (x.dtype, t.float32):
-        raise ValueError(f"out_dtype: {dtype} is neither {x.dtype} nor float32")
-    flip, ldw, group_stride = _groups(w)
-    off = offsets_device(offsets, g, rows, x.device)
-    scale, shift = _affine("scale", scale, g, n, x.device), _affine("shift", shift, g, n, x.device)
-    if scale is not None and shift is not None and scale.stride() != shift.stride():
-        scale, shift = scale.contiguous(), shift.contiguous()
-    some = scale if scale is not None else shift
-    if some is not None and n > 1 and some.stride(1) != 1:
-        scale, shift = (None if a is None else a.contiguous() for a in (scale, shift))
-        some = scale if scale is not None else shift
-    slope = float(slope)
+    t, types, L = _env()
+    _check_tensor(t, types, "x", x, 2, None, None)
+    xt, device = x.dtype, x.device
+    _check_tensor(t, types, "w", w, 3, xt, device)
+    rows, k = x.shape
+    g, wk, n, flip, ldw, group_stride = _weights("w", w, transposed)
+    if wk != k:
+        raise ValueError(f"x has {k} columns, the weight blocks have {wk} rows")
+    ldx = _row_stride("x", rows, k, *x.stride())
+    dtype = out_dtype or (xt if out is None else out.dtype)
+    if dtype is not xt and dtype is not t.float32:
+        raise ValueError(f"out_dtype: {dtype} is neither {xt} nor float32")
+    off = offsets_device(offsets, g, rows, device)
+    sc = sh = None
+    stride = 0
+    if scale is not None or shift is not None:
+        (sc, s1), (sh, s2) = ((None, None) if a is None else _affine(name, a, g, n, device) for name, a in (("scale", scale), ("shift", shift)))
+        if s1 is not None and s2 is not None and s1 != s2:            # one for all groups, the other for each
+            sc, sh, s1 = sc.expand(g, n).contiguous(), sh.expand(g, n).contiguous(), n
+        stride = s1 if s1 is not None else s2
     fill = out is None
-    with t.cuda.device(x.device):
-        if fill:
-            out = _dev.empty((rows, n), dtype, x.device)
-        else:
-            _check_matrix("out", out, 2, dtype, x.device)
-            if tuple(out.shape) != (rows, n):
-                raise ValueError(f"out: shape {tuple(out.shape)}, expected {(rows, n)}")
-            if any(_overlap(out, a) for a in (x, w)):
-                raise ValueError("out: overlaps x or w")
-        need = L.ct_grouped_product_workspace_bytes(_types()[x.dtype], rows, k, n, g)
-        ws = _dev.workspace(need, x.device) if need else None
-        _lib.check(L.ct_grouped_product(_types()[x.dtype], _types()[dtype], x.data_ptr(), _row_stride("x", x), rows, k, w.data_ptr(), group_stride, ldw,
-                                        int(flip), n, off.data_ptr(), g, None if scale is None else scale.data_ptr(),
-                                        None if shift is None else shift.data_ptr(), 0 if some is None or g == 1 else some.stride(0), slope, int(fill),
-                                        out.data_ptr(), _row_stride("out", out), None if ws is None else ws.data_ptr(), need, _dev.stream(x.device)),
-                   "ct_grouped_product")
+    if fill:
+        out, ldy = t.empty((rows, n), dtype=dtype, device=device), n
+    else:
+        _check_tensor(t, types, "out", out, 2, dtype, device)
+        if tuple(out.shape) != (rows, n):
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {(rows, n)}")
+        ldy = _row_stride("out", rows, n, *out.stride())
+        if _overlap(out, x) or _overlap(out, w):
+            raise ValueError("out: overlaps x or w")
+    with _On(t, device) as stream:
+        need = L.ct_grouped_product_workspace_bytes(types[xt], rows, k, n, g)
+        ws = _dev.workspace(need, device) if need else None
+        rc = L.ct_grouped_product(types[xt], types[dtype], x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n, off.data_ptr(), g,
+                                  sc.data_ptr() if sc is not None else None, sh.data_ptr() if sh is not None else None, stride, slope, fill,
+                                  out.data_ptr(), ldy, ws.data_ptr() if need else None, need, stream)
+    if rc:
+        _lib.check(rc, "ct_grouped_product")
     return out
 
 
@@ -157,28 +177,28 @@ def product_grad(dy, x, w, offsets, *, need_x: bool = True, need_w: bool = True,
     """The gradients of product(x, w, offsets) (no scale, shift or slope) for dy [rows, N] -> (dx [rows, K] of x's type, dw [G, K, N] of
     `out_dtype`: w's type, or float32); None in the place of one that is not needed.  Rows behind offsets[G] get a zero dx, a group without
     rows a zero dw[g].  Of a block that w.expand shares, each group's part comes separately: sum them."""
-    t = _lib.require_gpu(); L = _lib.lib()
-    _check_matrix("x", x, 2)
-    _check_matrix("w", w, 3, x.dtype, x.device)
-    _check_matrix("dy", dy, 2, x.dtype, x.device)
-    g, k, n = w.shape
-    rows = x.shape[0]
-    if tuple(dy.shape) != (rows, n) or x.shape[1] != k:
+    t, types, L = _env()
+    _check_tensor(t, types, "x", x, 2, None, None)
+    xt, device = x.dtype, x.device
+    _check_tensor(t, types, "w", w, 3, xt, device)
+    _check_tensor(t, types, "dy", dy, 2, xt, device)
+    rows, k = x.shape
+    g, wk, n, flip, ldw, group_stride = _weights("w", w, False)
+    if wk != k or tuple(dy.shape) != (rows, n):
         raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and w {tuple(w.shape)} do not fit each other")
-    if g < 1 or g > MAX_GROUPS or n < 1 or k < 1:
-        raise ValueError(f"w: shape {tuple(w.shape)} is empty or has more than {MAX_GROUPS} groups")
-    dtype = out_dtype or w.dtype
-    if dtype not in (w.dtype, t.float32):
-        raise ValueError(f"out_dtype: {dtype} is neither {w.dtype} nor float32")
-    off = offsets_device(offsets, g, rows, x.device)
-    dx = product(dy, w, off, transposed=True) if need_x else None
-    if not need_w:
-        return dx, None
-    with t.cuda.device(x.device):
-        dw = _dev.empty((g, k, n), dtype, x.device)
-        need = L.ct_grouped_product_dw_workspace_bytes(_types()[x.dtype], rows, k, n, g)
-        ws = _dev.workspace(need, x.device) if need else None
-        _lib.check(L.ct_grouped_product_dw(_types()[x.dtype], _types()[dtype], x.data_ptr(), _row_stride("x", x), rows, k, dy.data_ptr(),
-                                           _row_stride("dy", dy), n, off.data_ptr(), g, dw.data_ptr(), k * n, n,
-                                           None if ws is None else ws.data_ptr(), need, _dev.stream(x.device)), "ct_grouped_product_dw")
+    ldx, lddy = _row_stride("x", rows, k, *x.stride()), _row_stride("dy", rows, n, *dy.stride())
+    dtype = out_dtype or xt
+    if dtype is not xt and dtype is not t.float32:
+        raise ValueError(f"out_dtype: {dtype} is neither {xt} nor float32")
+    off = offsets_device(offsets, g, rows, device)
+    dx = t.empty((rows, k), dtype=xt, device=device) if need_x else None
+    dw = t.empty((g, k, n), dtype=dtype, device=device) if need_w else None
+    with _On(t, device) as stream:
+        need = L.ct_grouped_product_grad_workspace_bytes(types[xt], rows, k, n, g)
+        ws = _dev.workspace(need, device) if need else None
+        rc = L.ct_grouped_product_grad(types[xt], types[dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n,
+                                       off.data_ptr(), g, dx.data_ptr() if need_x else None, k, dw.data_ptr() if need_w else None, k * n, n,
+                                       ws.data_ptr() if need else None, need, stream)
+    if rc:
+        _lib.check(rc, "ct_grouped_product_grad")
     return dx, dw

@@ -67,6 +67,9 @@ CASES = [
     ([1], 1, 1, 0), ([1], 64, 64, 0), ([0, 1, 0], 61, 512, 0), ([5, 0, 0, 7], 3, 5, 2), ([64, 64], 64, 64, 0), ([65, 63, 1], 65, 129, 1),
     ([600, 613], 61, 512, 0), ([17], 512, 130, 3), ([0, 0, 0], 16, 16, 4), ([1] * 130, 48, 40, 0), ([3, 0] * 70, 33, 17, 9), ([300], 130, 1, 0),
     ([129, 2, 0, 258], 257, 255, 5), ([700, 1, 90], 128, 256, 0),
+    # the large tiles: more of them than compute units, partial in every direction
+    ([4000, 0, 3500, 777], 72, 2050, 3), ([2100, 1, 2300], 136, 1161, 0), ([0, 90, 64, 131, 77, 1, 200, 63, 65, 2], 1300, 1290, 1),
+    ([33, 0, 100, 5] * 4, 520, 517, 2), ([9] * 20 + [0] * 10 + [31], 700, 264, 2), ([40, 31], 2050, 70, 0),
 ]
 
 
@@ -296,13 +299,16 @@ def test_the_abi_refuses_without_a_gpu():
     ok = dict(type=0, out=0, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, sc=None, sh=None, ag=0, slope=1.0, fill=1, y=64, ldy=6,
               ws=None, wsb=0, st=None)
     call = lambda **kw: L.ct_grouped_product(*{**ok, **kw}.values())
-    for kw in (dict(type=3), dict(type=-1), dict(out=1), dict(rows=-1), dict(K=-1), dict(N=0), dict(G=0), dict(x=None), dict(w=None), dict(off=None), dict(y=None),
+    for kw in (dict(type=3), dict(type=-1), dict(out=1), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(w=None), dict(off=None), dict(y=None),
                dict(ldx=7), dict(ldw=5), dict(ldy=5), dict(wg=-1), dict(ag=-1), dict(wt=1, ldw=7)):
         assert call(**kw) == _lib.CT_EINVAL, kw
     assert call(rows=0) == 0
     assert call(rows=2 ** 31 - 1, N=2 ** 20, ldw=2 ** 20, ldy=2 ** 20) == _lib.CT_ESHAPE
-    ok2 = dict(type=0, out=0, x=64, ldx=8, rows=4, K=8, dy=64, lddy=6, N=6, off=64, G=2, dw=64, wg=48, ldw=6, ws=None, wsb=0, st=None)
-    call2 = lambda **kw: L.ct_grouped_product_dw(*{**ok2, **kw}.values())
-    for kw in (dict(type=3), dict(out=2), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(dy=None), dict(off=None), dict(dw=None), dict(ldx=7),
-               dict(lddy=5), dict(ldw=5), dict(wg=47)):
+    ok2 = dict(type=0, out=0, dy=64, lddy=6, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, dx=64, lddx=8, dw=64, dwg=48, lddw=6, ws=None,
+               wsb=0, st=None)
+    call2 = lambda **kw: L.ct_grouped_product_grad(*{**ok2, **kw}.values())
+    for kw in (dict(type=3), dict(out=2), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(dy=None), dict(w=None), dict(off=None), dict(ldx=7),
+               dict(lddy=5), dict(ldw=5), dict(lddw=5), dict(dwg=47), dict(lddx=7), dict(wg=-1), dict(wt=1, ldw=7)):
         assert call2(**kw) == _lib.CT_EINVAL, kw
+    for kw in (dict(ldx=2 ** 22 + 1), dict(lddy=2 ** 22 + 1), dict(ldw=2 ** 22 + 1)):
+        assert call2(**kw) == _lib.CT_ESHAPE, kw
