@@ -262,8 +262,8 @@ enum Way { DIRECT, REGS, EDGE };
 // one tile: acc[i][j] holds D = B^T A^T of strips (n strip i, m strip j): a lane has 4 neighbours along n of one m
 // ------------------------------------------------------------------------------------------------
 // WM x WN waves share the tile, WK of them each take a part of every stage's contraction steps (small tiles: more of a long sum in flight) and add
-// up through LDS at the end, in order.  Two stages in LDS, one in flight while the other is multiplied.
-template <typename TT, bool ACC, bool BCC, int BM, int BN, int BK, int WM, int WN, int WK, Way WAY>
+// up through LDS at the end, in order.  NB stages in LDS (2 through registers): NB - 1 are in flight while one is multiplied.
+template <typename TT, bool ACC, bool BCC, int BM, int BN, int BK, int WM, int WN, int WK, int NB, Way WAY>
 struct Core {
     typedef typename TT::S S;
     static constexpr bool H = sizeof(S) == 2;
@@ -272,7 +272,8 @@ struct Core {
     typedef Tile<S, ACC, BM, BK> TA;
     typedef Tile<S, BCC, BN, BK> TB;
     static constexpr int STAGE_BYTES = TA::BYTES + TB::BYTES, SUM_BYTES = WK > 1 ? BM * BN * WK * 4 : 0;
-    static constexpr int LDS_BYTES = 2 * STAGE_BYTES > SUM_BYTES ? 2 * STAGE_BYTES : SUM_BYTES;
+    static constexpr int LDS_BYTES = NB * STAGE_BYTES > SUM_BYTES ? NB * STAGE_BYTES : SUM_BYTES;
+    static_assert(WAY == DIRECT || NB == 2, "registers hold one stage");
     // fp32 sums of one wave run over at most kChain steps and are then added to the total: a long chain loses a bit for every fourfold length
     static constexpr int kChain = 512;
     static constexpr bool FOLD = !H && WK == 1;
@@ -310,118 +311,167 @@ struct Core {
         }
     }
 
-    // A, B: element (0 of the tile, contraction step 0 of the operand); m_have rows-or-columns of A and n_have of B exist from there, rows of them (where
-    // m or n is contiguous) have len_a, len_b values.  The steps [begin, end) of `extent` are summed.
-    __device__ __forceinline__ void run(unsigned char* smem, const S* A, uint32_t lda, int m_have, int len_a, const S* B, uint32_t ldb, int n_have, int len_b,
-                                        int begin, int end, int extent) {
-        int m0, n0, kz;
-        place(m0, n0, kz);
-        ra.init(m0, kz * PK); rb.init(n0, kz * PK);
-        f32x4 total[FOLD ? SN : 1][FOLD ? SM : 1];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < SN; ++i)
+#pragma unroll
+            for (int j = 0; j < SM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // Parts of the sum meet in LDS; wave kz goes on with every WK-th strip
+    __device__ __forceinline__ void join(unsigned char* smem, int kz) {
+        __syncthreads();
+        f32x4* const part = (f32x4*)smem;
+        const int lane = threadIdx.x & 63, mn = (threadIdx.x >> 6) % (WM * WN);
+#pragma unroll
+        for (int i = 0; i < SN; ++i)
+#pragma unroll
+            for (int j = 0; j < SM; ++j) part[((kz * WM * WN + mn) * SN * SM + i * SM + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < SN; ++i)
 #pragma unroll
             for (int j = 0; j < SM; ++j) {
-                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if constexpr (FOLD) total[i][j] = acc[i][j];
+                if ((i * SM + j) % WK != kz) continue;
+                f32x4 v = part[(mn * SN * SM + i * SM + j) * 64 + lane];
+#pragma unroll
+                for (int z = 1; z < WK; ++z) v += part[((z * WM * WN + mn) * SN * SM + i * SM + j) * 64 + lane];
+                acc[i][j] = v;
             }
+    }
+
+    // `tiles` tiles with the same A one after the other: tile i has B(i) -- element (0 of the tile, contraction step 0), n_have(i) rows-or-columns of it
+    // existing from there -- and done(i) takes its sums.  m_have rows-or-columns of A exist; rows of A and B (where m or n is contiguous) have
+    // len_a, len_b values.  The steps [begin, end) of `extent` are summed.  More than one tile only if MANY, with DIRECT and WK = 1.
+    template <bool MANY, typename FB, typename FN, typename FD>
+    __device__ __forceinline__ void run(unsigned char* smem, const S* A, uint32_t lda, int m_have, int len_a, int tiles, FB B, uint32_t ldb, FN n_have, int len_b,
+                                        int begin, int end, int extent, FD done) {
+        int m0, n0, kz;
+        place(m0, n0, kz);
+        ra.init(m0, kz * PK); rb.init(n0, kz * PK);
+        f32x4 total[FOLD ? SN : 1][FOLD ? SM : 1];
+        clear();
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < SN; ++i)
+#pragma unroll
+                for (int j = 0; j < SM; ++j) total[i][j] = acc[i][j];
+        }
         const int stages = (end - begin + BK - 1) / BK;
-        auto la = [&](int t) { return (S*)(smem + (t & 1) * STAGE_BYTES); };
-        auto lb = [&](int t) { return (S*)(smem + (t & 1) * STAGE_BYTES + TA::BYTES); };
+        const int full = WAY == EDGE ? stages : (end - begin) / BK;             // stages all of whose steps count; one more may follow
         auto from = [&](int t) { const int c = begin + t * BK; return WAY == EDGE || c + BK <= extent ? c : extent - BK; };
         auto pa = [&](int t) { return A + (ACC ? (int64_t)from(t) : (int64_t)from(t) * lda); };
-        auto pb = [&](int t) { return B + (BCC ? (int64_t)from(t) : (int64_t)from(t) * ldb); };
-        const int full = WAY == EDGE ? stages : (end - begin) / BK;             // stages all of whose steps count; one more may follow
-        auto step = [&](int t) {
-            multiply<false>(smem + (t & 1) * STAGE_BYTES, kz, 0, 0);
-            if constexpr (FOLD)
-                if ((t + 1) % (kChain / BK) == 0) {
+        auto pb = [&](int i, int t) { return B(i) + (BCC ? (int64_t)from(t) : (int64_t)from(t) * ldb); };
+        auto fold = [&] {
+            if constexpr (FOLD) {
 #pragma unroll
-                    for (int i = 0; i < SN; ++i)
+                for (int i = 0; i < SN; ++i)
 #pragma unroll
-                        for (int j = 0; j < SM; ++j) { total[i][j] += acc[i][j]; acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-                }
+                    for (int j = 0; j < SM; ++j) { total[i][j] += acc[i][j]; acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+            }
         };
-        auto last = [&](int t) { multiply<true>(smem + (t & 1) * STAGE_BYTES, kz, begin + t * BK - from(t), end - from(t)); };
+        auto step = [&](int t, int u) {
+            multiply<false>(smem + u % NB * STAGE_BYTES, kz, 0, 0);
+            if constexpr (FOLD) if ((t + 1) % (kChain / BK) == 0) fold();
+        };
+        auto last = [&](int t, int u) { multiply<true>(smem + u % NB * STAGE_BYTES, kz, begin + t * BK - from(t), end - from(t)); };
+        auto finish = [&](int i) {
+            if constexpr (FOLD) {
+#pragma unroll
+                for (int a = 0; a < SN; ++a)
+#pragma unroll
+                    for (int b = 0; b < SM; ++b) { acc[a][b] += total[a][b]; total[a][b] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+            }
+            if constexpr (WK > 1) join(smem, kz);
+            done(i);
+        };
+        static_assert(!MANY || (WAY == DIRECT && WK == 1), "the sums of one tile are joined where the next one's stages would stand");
         if constexpr (WAY == DIRECT) {
             Direct<S, ACC, BM, BK, NT> da;
             Direct<S, BCC, BN, BK, NT> db;
-            da.init(lda, m_have); db.init(ldb, n_have);
+            da.init(lda, m_have); db.init(ldb, n_have(0));
             const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-            auto issue = [&](int t) {
-                da.load(pa(t), lds + (t & 1) * STAGE_BYTES);
-                db.load(pb(t), lds + (t & 1) * STAGE_BYTES + TA::BYTES);
+            const int all = MANY ? tiles * stages : stages;
+            int ti = 0, tt = 0;                                                 // the next stage to ask for: of tile ti its stage tt
+            auto issue = [&](int u) {
+                if (!MANY) tt = u;
+                da.load(pa(tt), lds + u % NB * STAGE_BYTES);
+                db.load(pb(ti, tt), lds + u % NB * STAGE_BYTES + TA::BYTES);
+                if (MANY && ++tt == stages) { tt = 0; ++ti; }
             };
-            if (stages > 0) issue(0);
-            auto landed = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };   // stage t is there, stage t - 1 has been read
-            for (int t = 0; t < full; ++t) {
-                landed();
-                if (t + 1 < stages) issue(t + 1);
-                step(t);
+            // stage u is there and stage u - 1 has been read by all; of the stages after u, those that have been asked for may still be on their way
+            auto landed = [&](int u) {
+                constexpr int AHEAD = (NB - 2) * (decltype(da)::N + decltype(db)::N);
+                static_assert(AHEAD < 64, "the counter of loads in flight has 6 bits");
+                if (NB > 2 && u + NB - 2 < all) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(AHEAD) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            };
+#pragma unroll
+            for (int u = 0; u < NB - 1; ++u) if (u < all) issue(u);
+            auto sum = [&](int u) {                                             // the stages of one tile, the first of them u
+                for (int t = 0; t < full; ++t, ++u) {
+                    landed(u);
+                    if (u + NB - 1 < all) issue(u + NB - 1);
+                    step(t, u);
+                }
+                if (full < stages) {
+                    landed(u);
+                    if (u + NB - 1 < all) issue(u + NB - 1);
+                    last(full, u);
+                }
+            };
+            if constexpr (MANY) {
+                for (int i = 0; i < tiles; ++i) {
+                    if (i) clear();
+                    sum(i * stages);
+                    finish(i);
+                    __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt(0), said so that the compiler does not put it among the next tile's reads
+                }
+            } else {
+                sum(0);
+                finish(0);
             }
-            if (full < stages) { landed(); last(full); }
         } else {
+            auto la = [&](int t) { return (S*)(smem + t % NB * STAGE_BYTES); };
+            auto lb = [&](int t) { return (S*)(smem + t % NB * STAGE_BYTES + TA::BYTES); };
             Stage<S, ACC, BM, BK, NT, WAY == EDGE> sa;
             Stage<S, BCC, BN, BK, NT, WAY == EDGE> sb;
+            const int n = n_have(0);
             auto load = [&](int t) {
                 const int c = end - from(t);
                 sa.load(pa(t), lda, ACC ? m_have : c, ACC ? c : m_have, ACC ? extent : len_a);
-                sb.load(pb(t), ldb, BCC ? n_have : c, BCC ? c : n_have, BCC ? extent : len_b);
+                sb.load(pb(0, t), ldb, BCC ? n : c, BCC ? c : n, BCC ? extent : len_b);
             };
             auto store = [&](int t) {
                 const int c = end - from(t);
                 sa.store(la(t), ACC ? m_have : c, ACC ? c : m_have, ACC ? extent : len_a);
-                sb.store(lb(t), BCC ? n_have : c, BCC ? c : n_have, BCC ? extent : len_b);
+                sb.store(lb(t), BCC ? n : c, BCC ? c : n, BCC ? extent : len_b);
             };
             if (stages > 0) { load(0); store(0); }
             __syncthreads();
             for (int t = 0; t < full; ++t) {
                 if (t + 1 < stages) load(t + 1);
-                step(t);
+                step(t, t);
                 if (t + 1 < stages) store(t + 1);
                 __syncthreads();
             }
-            if (full < stages) last(full);
-        }
-        if constexpr (FOLD) {
-#pragma unroll
-            for (int i = 0; i < SN; ++i)
-#pragma unroll
-                for (int j = 0; j < SM; ++j) acc[i][j] += total[i][j];
-        }
-        if constexpr (WK > 1) {                                 // parts of the sum meet in LDS; wave kz goes on with every WK-th strip
-            __syncthreads();
-            f32x4* const part = (f32x4*)smem;
-            const int lane = threadIdx.x & 63, mn = (threadIdx.x >> 6) % (WM * WN);
-#pragma unroll
-            for (int i = 0; i < SN; ++i)
-#pragma unroll
-                for (int j = 0; j < SM; ++j) part[((kz * WM * WN + mn) * SN * SM + i * SM + j) * 64 + lane] = acc[i][j];
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < SN; ++i)
-#pragma unroll
-                for (int j = 0; j < SM; ++j) {
-                    if ((i * SM + j) % WK != kz) continue;
-                    f32x4 v = part[(mn * SN * SM + i * SM + j) * 64 + lane];
-#pragma unroll
-                    for (int z = 1; z < WK; ++z) v += part[((z * WM * WN + mn) * SN * SM + i * SM + j) * 64 + lane];
-                    acc[i][j] = v;
-                }
+            if (full < stages) last(full, full);
+            finish(0);
         }
     }
-    // f(m, n, four neighbours along n)
-    template <typename F> __device__ __forceinline__ void each(F f) const {
+    // for each column strip: col(n), then row(m, n, four neighbours along n)
+    template <typename C, typename R> __device__ __forceinline__ void each(C col, R row) const {
         const int lane = threadIdx.x & 63, l16 = lane & 15, lk = lane >> 4;
         int m0, n0, kz;
         place(m0, n0, kz);
 #pragma unroll
-        for (int j = 0; j < SM; ++j)
+        for (int i = 0; i < SN; ++i) {
+            col(n0 + 16 * i + 4 * lk);
 #pragma unroll
-            for (int i = 0; i < SN; ++i) {
+            for (int j = 0; j < SM; ++j) {
                 if (WK > 1 && (i * SM + j) % WK != kz) continue;
-                f(m0 + 16 * j + l16, n0 + 16 * i + 4 * lk, acc[i][j]);
+                row(m0 + 16 * j + l16, n0 + 16 * i + 4 * lk, acc[i][j]);
             }
+        }
     }
 };
 
@@ -433,6 +483,14 @@ __device__ __forceinline__ void store4(O* p, f32x4 v, int first, int have) {   /
     for (int i = 0; i < 4; ++i) if (i >= first && i < have) p[i] = r[i];
 }
 // out: CT_F32 or the operands' type
+__device__ __forceinline__ f32x4 load4(const float* p, int n, int have) {       // 4 neighbours; those past `have` repeat the last one
+    typedef f32x4 loose4 __attribute__((aligned(4)));
+    if (n + 4 <= have) return *reinterpret_cast<const loose4*>(p + n);
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[n + i < have ? n + i : have - 1];
+    return v;
+}
 template <typename S>
 __device__ __forceinline__ void store_out(void* p, int64_t at, bool f32, f32x4 v, int first, int have) {
     if (sizeof(S) == 4 || f32) store4((float*)p + at, v, first, have); else store4((S*)p + at, v, first, have);
@@ -454,50 +512,60 @@ struct ProductP {
     const float* scale; const float* shift; int64_t ag; float slope;
     int tail, out32;
     void* y; int64_t ldy;
-    int slots, nt, count;                    // row tiles (at most), column tiles, workgroups
+    int slots, nt, per, count;               // row tiles (at most), runs of column tiles, column tiles in a run (at most), workgroups
 };
 
 // The last column tile is moved back so that it ends with the matrix (its first columns are then another tile's to store): whole pieces in every tile.
 __device__ __forceinline__ int moved_back(int at, int tile, int extent) { return at + tile <= extent || extent < tile ? at : extent - tile; }
 
-template <typename TT, bool WT, int BM, int BN, int BK, int WM, int WN, int WK, Way WAY>
-__global__ __launch_bounds__(64 * WM * WN * WK) void product_kernel(const ProductP p) {
+// A tile's shape and how it is worked: what Core is made of
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int WK_, int NB_, Way WAY_, int RUN_ = 1>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, BK = BK_, NB = NB_, RUN = RUN_, THREADS = 64 * WM_ * WN_ * WK_, WK = WK_;
+    static constexpr Way WAY = WAY_;
+    template <typename TT, bool ACC, bool BCC> using Of = Core<TT, ACC, BCC, BM_, BN_, BK_, WM_, WN_, WK_, NB_, WAY_>;
+};
+
+template <typename TT, bool WT, typename Sh>
+__device__ __forceinline__ void product_tile(const ProductP& p, int id, unsigned char* smem) {
     typedef typename TT::S S;
-    typedef Core<TT, true, WT, BM, BN, BK, WM, WN, WK, WAY> C;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS_BYTES];
+    typedef typename Sh::template Of<TT, true, WT> C;
+    constexpr int BM = Sh::BM, BN = Sh::BN;
     // four row tiles side by side, then the next column tile: 32 numbers in a row touch 4 row panels and 8 column panels
-    const int t = tile_number(blockIdx.x, p.count), strip = 4 * p.nt, s4 = t / strip, in = t - s4 * strip;
+    const int t = tile_number(id, p.count), strip = 4 * p.nt, s4 = t / strip, in = t - s4 * strip;
     const int wide = p.slots - 4 * s4 < 4 ? p.slots - 4 * s4 : 4, col = in / wide, slot = 4 * s4 + in - col * wide;
     const Slot s = find_slot(p.off, p.G, p.rows, BM, slot, p.tail);
     if (s.group < 0) return;
-    const int nom = col * BN, n0 = moved_back(nom, BN, p.N), first = nom - n0;
-    const int m_have = s.end - s.row, n_have = p.N - n0;
-    const int64_t at = (int64_t)s.row * p.ldy + n0;
+    const int m_have = s.end - s.row, c0 = col * p.per, cols = (p.N + BN - 1) / BN, runs = cols - c0 < p.per ? cols - c0 : p.per;
     if (s.group == p.G) {                    // rows behind the last group
-        for (int i = threadIdx.x; i < BM * (BN / 4); i += C::NT) {
-            const int m = i / (BN / 4), n = i % (BN / 4) * 4;
-            if (m < m_have && n < n_have) store_out<S>(p.y, at + m * p.ldy + n, p.out32, f32x4{0.f, 0.f, 0.f, 0.f}, first - n, n_have - n);
+        const int n0 = c0 * BN, wide = p.N - n0 < runs * BN ? p.N - n0 : runs * BN, quads = (wide + 3) / 4;
+        for (int i = threadIdx.x; i < BM * quads; i += C::NT) {
+            const int m = i / quads, n = i % quads * 4;
+            if (m < m_have) store_out<S>(p.y, (int64_t)(s.row + m) * p.ldy + n0 + n, p.out32, f32x4{0.f, 0.f, 0.f, 0.f}, 0, wide - n);
         }
         return;
     }
-    const S* const w = (const S*)p.w + s.group * p.wg + (WT ? n0 * p.ldw : (int64_t)n0);
+    const S* const w = (const S*)p.w + s.group * p.wg;
+    const float* const sc = p.scale ? p.scale + s.group * p.ag : nullptr;
+    const float* const sh = p.shift ? p.shift + s.group * p.ag : nullptr;
+    auto begins = [&](int i) { return moved_back((c0 + i) * BN, BN, p.N); };
     C core;
-    core.run(smem, (const S*)p.x + (int64_t)s.row * p.ldx, (uint32_t)p.ldx, m_have, p.K, w, (uint32_t)p.ldw, n_have, p.N, 0, p.K, p.K);
-    const float* const sc = p.scale ? p.scale + s.group * p.ag + n0 : nullptr;
-    const float* const sh = p.shift ? p.shift + s.group * p.ag + n0 : nullptr;
-    core.each([&](int m, int n, f32x4 v) {
-        if (m >= m_have || n >= n_have) return;
-        if (sc || sh) {
+    core.template run<(Sh::RUN > 1)>(smem, (const S*)p.x + (int64_t)s.row * p.ldx, (uint32_t)p.ldx, m_have, p.K, runs,
+             [&](int i) { return w + (WT ? begins(i) * p.ldw : (int64_t)begins(i)); }, (uint32_t)p.ldw, [&](int i) { return p.N - begins(i); }, p.N, 0, p.K, p.K, [&](int i) {
+        const int n0 = begins(i), first = (c0 + i) * BN - n0, n_have = p.N - n0;
+        const int64_t at = (int64_t)s.row * p.ldy + n0;
+        f32x4 a = {1.f, 1.f, 1.f, 1.f}, b = {0.f, 0.f, 0.f, 0.f};
+        core.each([&](int n) {
+            if (sc) a = load4(sc + n0, n, n_have);
+            if (sh) b = load4(sh + n0, n, n_have);
+        }, [&](int m, int n, f32x4 v) {
+            if (m >= m_have || n >= n_have) return;
+            if (sc) v *= a;
+            if (sh) v += b;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int ni = n + i < n_have ? n + i : n_have - 1;
-                if (sc) v[i] *= sc[ni];
-                if (sh) v[i] += sh[ni];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = v[i] >= 0.f ? v[i] : v[i] * p.slope;
-        store_out<S>(p.y, at + m * p.ldy + n, p.out32, v, first - n, n_have - n);
+            for (int k = 0; k < 4; ++k) v[k] = v[k] >= 0.f ? v[k] : v[k] * p.slope;
+            store_out<S>(p.y, at + m * p.ldy + n, p.out32, v, first - n, n_have - n);
+        });
     });
 }
 
@@ -509,109 +577,216 @@ struct DwP {
     int out32, mt, nt, count;
 };
 
-template <typename TT, int BM, int BN, int BK, int WM, int WN, int WK, Way WAY>
-__global__ __launch_bounds__(64 * WM * WN * WK) void dw_kernel(const DwP p) {
+template <typename TT, typename Sh>
+__device__ __forceinline__ void dw_tile(const DwP& p, int id, unsigned char* smem) {
     typedef typename TT::S S;
-    typedef Core<TT, false, false, BM, BN, BK, WM, WN, WK, WAY> C;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS_BYTES];
-    const int tile = tile_number(blockIdx.x, p.count), g = tile / (p.mt * p.nt), t = tile - g * p.mt * p.nt;
+    typedef typename Sh::template Of<TT, false, false> C;
+    constexpr int BM = Sh::BM, BN = Sh::BN;
+    const int tile = tile_number(id, p.count), g = tile / (p.mt * p.nt), t = tile - g * p.mt * p.nt;
     const int nom_m = (t / p.nt) * BM, m0 = moved_back(nom_m, BM, p.K), nom_n = (t % p.nt) * BN, n0 = moved_back(nom_n, BN, p.N);
     const int b = clampi(fresh_i32(p.off + g), 0, p.rows), e = clampi(fresh_i32(p.off + g + 1), b, p.rows);
     C core;
-    core.run(smem, (const S*)p.x + m0, (uint32_t)p.ldx, p.K - m0, p.K, (const S*)p.dy + n0, (uint32_t)p.lddy, p.N - n0, p.N, b, e, p.rows);
+    core.template run<false>(smem, (const S*)p.x + m0, (uint32_t)p.ldx, p.K - m0, p.K, 1, [&](int) { return (const S*)p.dy + n0; }, (uint32_t)p.lddy, [&](int) { return p.N - n0; }, p.N, b, e,
+             p.rows, [](int) {});
     const int64_t at = g * p.wg + m0 * p.ldw + n0;
-    core.each([&](int m, int n, f32x4 v) {
+    core.each([](int) {}, [&](int m, int n, f32x4 v) {
         if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store_out<S>(p.dw, at + m * p.ldw + n, p.out32, v, nom_n - n0 - n, p.N - n0 - n);
     });
 }
 
+template <typename TT, bool WT, typename Sh>
+__global__ __launch_bounds__(Sh::THREADS) void product_kernel(const ProductP p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Sh::template Of<TT, true, WT>::LDS_BYTES];
+    product_tile<TT, WT, Sh>(p, blockIdx.x, smem);
+}
+template <typename TT, typename Sh>
+__global__ __launch_bounds__(Sh::THREADS) void dw_kernel(const DwP p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Sh::template Of<TT, false, false>::LDS_BYTES];
+    dw_tile<TT, Sh>(p, blockIdx.x, smem);
+}
+// Both gradients in one launch: neither alone fills the card at the sizes of a network's layers, and one launch costs as much as a small product
+template <typename TT, bool WT, typename ShX, typename ShW>
+__global__ __launch_bounds__(ShX::THREADS) void grad_kernel(const ProductP x, const DwP w, int w_first) {
+    constexpr int LX = ShX::template Of<TT, true, WT>::LDS_BYTES, LW = ShW::template Of<TT, false, false>::LDS_BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[LX > LW ? LX : LW];
+    const int id = blockIdx.x, ahead = w_first ? w.count : x.count;
+    if ((id < ahead) == (w_first != 0)) dw_tile<TT, ShW>(w, w_first ? id : id - ahead, smem);
+    else product_tile<TT, WT, ShX>(x, w_first ? id - ahead : id, smem);
+}
+
 constexpr int64_t kMaxBlocks = (1 << 22) - 1;               // a grid has fewer than 2^32 work items, a workgroup up to 512
 constexpr int64_t kMaxStride = 1 << 22;                     // a tile's offsets fit 32 bits: 256 rows of 2^22 values
+constexpr int64_t kCus = 256;
 
 bool type_ok(int t) { return t == CT_F32 || t == CT_BF16 || t == CT_F16; }
 bool words(const void* p, int64_t ld, int64_t more, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size) | (uintptr_t)(more * size)) & 3) == 0; }
+int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
-template <typename TT, bool WT, int BM, int BN, int BK, int WM, int WN, int WK, Way WAY>
-int product_launch(ProductP p, hipStream_t st) {
-    p.nt = (p.N + BN - 1) / BN;
-    const int64_t slots = (int64_t)p.rows / BM + (p.rows < p.G + 1 ? p.rows : p.G + 1);     // sum of ceil(rows_g / BM) is no more
+// Workgroups of a launch; CT_ESHAPE: too many; CT_EINVAL: a tile would reach outside its operands, which the rules below never ask for
+template <bool WT, typename Sh>
+int plan(ProductP& p) {
+    if (Sh::WAY != EDGE && (p.K < Sh::BK || (!WT && p.N < Sh::BN))) return CT_EINVAL;
+    const int cols = (p.N + Sh::BN - 1) / Sh::BN;
+    p.per = Sh::RUN < cols ? Sh::RUN : cols;
+    p.nt = (cols + p.per - 1) / p.per;
+    const int64_t slots = (int64_t)p.rows / Sh::BM + (p.rows < p.G + 1 ? p.rows : p.G + 1);     // sum of ceil(rows_g / BM) is no more
     if (slots * p.nt > kMaxBlocks) return CT_ESHAPE;
     p.slots = (int)slots; p.count = (int)(slots * p.nt);
-    hipLaunchKernelGGL((product_kernel<TT, WT, BM, BN, BK, WM, WN, WK, WAY>), dim3((unsigned)p.count), dim3(64 * WM * WN * WK), 0, st, p);
-    return (int)hipGetLastError();
+    return CT_OK;
 }
-template <typename TT, int BM, int BN, int BK, int WM, int WN, int WK, Way WAY>
-int dw_launch(DwP p, hipStream_t st) {
-    p.mt = (p.K + BM - 1) / BM; p.nt = (p.N + BN - 1) / BN;
+template <typename Sh>
+int plan(DwP& p) {
+    if (Sh::WAY != EDGE && (p.rows < Sh::BK || p.K < Sh::BM || p.N < Sh::BN)) return CT_EINVAL;
+    p.mt = (p.K + Sh::BM - 1) / Sh::BM; p.nt = (p.N + Sh::BN - 1) / Sh::BN;
     const int64_t count = (int64_t)p.G * p.mt * p.nt;
     if (count > kMaxBlocks) return CT_ESHAPE;
     p.count = (int)count;
-    hipLaunchKernelGGL((dw_kernel<TT, BM, BN, BK, WM, WN, WK, WAY>), dim3((unsigned)p.count), dim3(64 * WM * WN * WK), 0, st, p);
+    return CT_OK;
+}
+template <typename TT, bool WT, typename Sh>
+int launch(ProductP p, hipStream_t st) {
+    const int rc = plan<WT, Sh>(p);
+    if (rc != CT_OK) return rc;
+    hipLaunchKernelGGL((product_kernel<TT, WT, Sh>), dim3((unsigned)p.count), dim3(Sh::THREADS), 0, st, p);
+    return (int)hipGetLastError();
+}
+template <typename TT, typename Sh>
+int launch(DwP p, hipStream_t st) {
+    const int rc = plan<Sh>(p);
+    if (rc != CT_OK) return rc;
+    hipLaunchKernelGGL((dw_kernel<TT, Sh>), dim3((unsigned)p.count), dim3(Sh::THREADS), 0, st, p);
+    return (int)hipGetLastError();
+}
+template <typename TT, bool WT, typename ShX, typename ShW>
+int launch(ProductP x, DwP w, hipStream_t st) {
+    static_assert(ShX::THREADS == ShW::THREADS, "one launch");
+    int rc = plan<WT, ShX>(x);
+    if (rc == CT_OK) rc = plan<ShW>(w);
+    if (rc != CT_OK) return rc;
+    if ((int64_t)x.count + w.count > kMaxBlocks) return CT_ESHAPE;
+    const int w_first = (int64_t)w.rows > (int64_t)w.G * x.K;       // the longer sums begin first: mean rows of a group against the width of dy
+    hipLaunchKernelGGL((grad_kernel<TT, WT, ShX, ShW>), dim3((unsigned)(x.count + w.count)), dim3(ShX::THREADS), 0, st, x, w, w_first);
     return (int)hipGetLastError();
 }
 
-constexpr int64_t kCus = 256;
-int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
+// Shapes.  Named by their tile; measured (us) at the sizes given with the rules.
+template <Way W> using T256 = Shape<256, 256, 64, 2, 4, 1, 2, W>;
+template <Way W> using T128 = Shape<128, 128, 64, 2, 4, 1, 2, W>;
+using T128run = Shape<128, 128, 64, 2, 4, 1, 2, DIRECT, 4>;
+using T128deep = Shape<128, 128, 64, 2, 4, 1, 4, DIRECT>;
+template <Way W> using T64 = Shape<64, 64, 64, 2, 2, 1, 2, W>;
+using T64deep = Shape<64, 64, 64, 2, 2, 1, 4, DIRECT>;
+template <Way W> using T64flat = Shape<64, 64, 32, 2, 2, 1, 2, W>;
+using T32 = Shape<32, 64, 128, 1, 2, 2, 2, DIRECT>;
+using T16 = Shape<16, 64, 256, 1, 1, 4, 2, DIRECT>;
+using T16r = Shape<16, 64, 128, 1, 1, 4, 2, REGS>;
+using F128 = Shape<128, 128, 32, 2, 4, 1, 2, DIRECT>;
+using F64 = Shape<64, 64, 32, 2, 2, 1, 2, DIRECT>;
+using F32 = Shape<32, 64, 64, 1, 1, 4, 2, DIRECT>;
+using F32s = Shape<32, 32, 64, 1, 1, 4, 2, DIRECT>;
+using F16 = Shape<16, 64, 128, 1, 1, 4, 2, DIRECT>;
+using Any = Shape<64, 64, 32, 2, 2, 1, 2, EDGE>;
 
 // Which tile.  16 x 64: a few rows a group, bound by the weights, every wave a quarter of the sum.  Large tiles where there are enough of them for all
-// CUs, since each value of an operand is then fetched less often; else small ones, with the sum split over the waves.
+// CUs, since each value of an operand is then fetched less often; else small ones.
 template <typename TT, bool WT, Way WAY>
 int product_pick(const ProductP& p, hipStream_t st) {
-    const int64_t mean = (p.rows + p.G - 1) / p.G, r = p.rows;
+    const int64_t mean = (p.rows + p.G - 1) / p.G, r = p.rows + p.G * 32;       // (a group's last tile is half full on average)
     const int k = p.K, n = WT ? 1 << 30 : p.N;              // what the tile must not exceed: rows of w may be repeated, columns may not
-    if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
-        constexpr int WIDE = WAY == DIRECT ? 256 : 128;
-        if (mean <= 16 && k >= WIDE && n >= 64) return product_launch<TT, WT, 16, 64, WIDE, 1, 1, 4, WAY>(p, st);
-        if constexpr (WAY == DIRECT)
-            if (mean >= 192 && k >= 64 && p.N >= 256 && tiles(r, p.N, 256, 256) >= kCus) return product_launch<TT, WT, 256, 256, 64, 2, 4, 1, WAY>(p, st);
-        if (mean >= 96 && k >= 64 && p.N >= 128 && tiles(r, p.N, 128, 128) >= kCus) return product_launch<TT, WT, 128, 128, 64, 2, 2, 1, WAY>(p, st);
-        if (k >= 128 && n >= 64) return product_launch<TT, WT, 64, 64, 128, 1, 2, 2, WAY>(p, st);
-        if (k >= 32 && n >= 64) return product_launch<TT, WT, 64, 64, 32, 2, 2, 1, WAY>(p, st);
+    if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2) {
+        const int64_t t128 = tiles(r, p.N, 128, 128), t64 = tiles(r, p.N, 64, 64);
+        if (mean <= 16 && k >= 256 && n >= 64) return launch<TT, WT, T16>(p, st);
+        if (mean >= 192 && k >= 64 && p.N >= 256 && tiles(r, p.N, 256, 256) >= kCus) return launch<TT, WT, T256<DIRECT>>(p, st);
+        if (mean >= 96 && k >= 64 && p.N >= 128 && t128 >= kCus) return k <= 128 && t128 >= 4 * kCus ? launch<TT, WT, T128run>(p, st) : launch<TT, WT, T128<DIRECT>>(p, st);
+        if (mean >= 96 && k >= 256 && p.N >= 128 && t128 >= 160) return launch<TT, WT, T128deep>(p, st);
+        if (k >= 128 && n >= 64 && t64 < 160) return launch<TT, WT, T32>(p, st);
+        if (k >= 256 && n >= 64 && t64 <= 2 * kCus) return launch<TT, WT, T64deep>(p, st);
+        if (k >= 64 && n >= 64) return launch<TT, WT, T64<DIRECT>>(p, st);
+        if (k >= 32 && n >= 64) return launch<TT, WT, T64flat<DIRECT>>(p, st);
+    }
+    if constexpr (WAY == REGS && sizeof(typename TT::S) == 2) {
+        if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, T16r>(p, st);
+        if (mean >= 96 && k >= 64 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 160) return launch<TT, WT, T128<REGS>>(p, st);
+        if (k >= 64 && n >= 64) return launch<TT, WT, T64<REGS>>(p, st);
+        if (k >= 32 && n >= 64) return launch<TT, WT, T64flat<REGS>>(p, st);
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
-        if (mean <= 16 && k >= 128 && n >= 64) return product_launch<TT, WT, 16, 64, 128, 1, 1, 4, WAY>(p, st);
-        if (mean >= 96 && k >= 32 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 2 * kCus) return product_launch<TT, WT, 128, 128, 32, 2, 2, 1, WAY>(p, st);
-        if (k >= 128 && n >= 32 && tiles(r, p.N, 64, 64) < 2 * kCus) return product_launch<TT, WT, 32, 32, 128, 1, 1, 4, WAY>(p, st);
-        if (k >= 32 && n >= 64) return product_launch<TT, WT, 64, 64, 32, 2, 2, 1, WAY>(p, st);
+        const int64_t t64 = tiles(r, p.N, 64, 64);
+        if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, F16>(p, st);
+        if (mean >= 96 && k >= 32 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 2 * kCus) return launch<TT, WT, F128>(p, st);
+        if (k >= 64 && n >= 64 && t64 < 2 * kCus && t64 >= kCus) return launch<TT, WT, F32>(p, st);
+        if (k >= 64 && n >= 32 && t64 < kCus) return launch<TT, WT, F32s>(p, st);
+        if (k >= 32 && n >= 64) return launch<TT, WT, F64>(p, st);
     }
-    return product_launch<TT, WT, 64, 64, 32, 2, 2, 1, EDGE>(p, st);
+    return launch<TT, WT, Any>(p, st);
 }
 template <typename TT, Way WAY>
 int dw_pick(const DwP& p, hipStream_t st) {
     const int r = p.rows, k = p.K, n = p.N;
     if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
         if constexpr (WAY == DIRECT)
-            if (r >= 64 && k >= 256 && n >= 256 && p.G * tiles(k, n, 256, 256) >= kCus) return dw_launch<TT, 256, 256, 64, 2, 4, 1, WAY>(p, st);
-        if (r >= 64 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= kCus) return dw_launch<TT, 128, 128, 64, 2, 2, 1, WAY>(p, st);
-        if (r >= 128 && k >= 64 && n >= 64) return dw_launch<TT, 64, 64, 128, 1, 2, 2, WAY>(p, st);
+            if (r >= 64 && k >= 256 && n >= 256 && p.G * tiles(k, n, 256, 256) >= kCus) return launch<TT, T256<WAY>>(p, st);
+        if (r >= 64 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= 160) return launch<TT, T128<WAY>>(p, st);
+        if (r >= 64 && k >= 64 && n >= 64) return launch<TT, T64<WAY>>(p, st);
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
-        if (r >= 32 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= 2 * kCus) return dw_launch<TT, 128, 128, 32, 2, 2, 1, WAY>(p, st);
-        if (r >= 128 && k >= 32 && n >= 32 && p.G * tiles(k, n, 64, 64) < 2 * kCus) return dw_launch<TT, 32, 32, 128, 1, 1, 4, WAY>(p, st);
-        if (r >= 32 && k >= 64 && n >= 64) return dw_launch<TT, 64, 64, 32, 2, 2, 1, WAY>(p, st);
+        if (r >= 32 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= 2 * kCus) return launch<TT, F128>(p, st);
+        if (r >= 64 && k >= 32 && n >= 32 && p.G * tiles(k, n, 64, 64) < 2 * kCus) return launch<TT, F32s>(p, st);
+        if (r >= 32 && k >= 64 && n >= 64) return launch<TT, F64>(p, st);
     }
-    return dw_launch<TT, 64, 64, 32, 2, 2, 1, EDGE>(p, st);
+    return launch<TT, Any>(p, st);
+}
+// Both gradients together where one shape suits them; x: dx as a product (its K is the width of dy, its N the width of x)
+template <typename TT, bool WT, Way WAY>
+int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
+    const int64_t mean = (x.rows + x.G - 1) / x.G, r = x.rows + x.G * 32;
+    auto sum = [&](int t) { return tiles(r, x.N, t, t) + w.G * tiles(w.K, w.N, t, t); };
+    const int least = w.K < w.N ? w.K : w.N;                // both widths bound a tile of dw
+    if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2)
+        if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return launch<TT, WT, T256<WAY>, T256<WAY>>(x, w, st);
+    if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
+        if (mean >= 96 && least >= 128 && sum(128) >= kCus) return launch<TT, WT, T128<WAY>, T128<WAY>>(x, w, st);
+        if (mean > 16 && x.rows >= 64 && least >= 64) return launch<TT, WT, T64<WAY>, T64<WAY>>(x, w, st);
+    }
+    if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
+        if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
+        if (mean > 16 && x.rows >= 64 && least >= 64) return sum(64) >= 2 * kCus ? launch<TT, WT, F64, F64>(x, w, st) : launch<TT, WT, F32, F32s>(x, w, st);
+    }
+    const int rc = dw_pick<TT, WAY>(w, st);
+    return rc == CT_OK ? product_pick<TT, WT, WAY>(x, st) : rc;
 }
 
-// direct loads want addresses that are multiples of 4 bytes (16-bit values: an even stride, and an even width where the last tile is moved back)
+// direct loads want addresses that are multiples of 4 bytes (16-bit values: an even stride, and an even width where the last tile is moved back);
+// fp32 always has them
+template <typename TT> constexpr Way other() { return sizeof(typename TT::S) == 2 ? REGS : DIRECT; }
 template <typename TT>
 int product_run(const ProductP& p, bool wt, hipStream_t st) {
     constexpr int size = sizeof(typename TT::S);
-    if (size == 4 || (words(p.x, p.ldx, p.K, size) && words(p.w, p.ldw, p.wg, size) && (wt || p.N % 2 == 0)))
-        return wt ? product_pick<TT, true, DIRECT>(p, st) : product_pick<TT, false, DIRECT>(p, st);
-    return wt ? product_pick<TT, true, size == 2 ? REGS : EDGE>(p, st) : product_pick<TT, false, size == 2 ? REGS : EDGE>(p, st);
+    const bool direct = words(p.x, p.ldx, p.K, size) && words(p.w, p.ldw, p.wg, size) && (wt || p.N % 2 == 0);
+    if (size == 4 || direct) return wt ? product_pick<TT, true, DIRECT>(p, st) : product_pick<TT, false, DIRECT>(p, st);
+    return wt ? product_pick<TT, true, other<TT>()>(p, st) : product_pick<TT, false, other<TT>()>(p, st);
 }
 template <typename TT>
 int dw_run(const DwP& p, hipStream_t st) {
     constexpr int size = sizeof(typename TT::S);
     if (size == 4 || (words(p.x, p.ldx, p.K, size) && words(p.dy, p.lddy, p.N, size))) return dw_pick<TT, DIRECT>(p, st);
-    return dw_pick<TT, size == 2 ? REGS : EDGE>(p, st);
+    return dw_pick<TT, other<TT>()>(p, st);
+}
+template <typename TT>
+int grad_run(const ProductP& x, const DwP& w, bool wt, hipStream_t st) {
+    constexpr int size = sizeof(typename TT::S);
+    const bool direct = words(w.x, w.ldx, w.K, size) && words(w.dy, w.lddy, w.N, size) && words(x.w, x.ldw, x.wg, size);
+    if (size == 4 || direct) return wt ? grad_pick<TT, true, DIRECT>(x, w, st) : grad_pick<TT, false, DIRECT>(x, w, st);
+    return wt ? grad_pick<TT, true, other<TT>()>(x, w, st) : grad_pick<TT, false, other<TT>()>(x, w, st);
 }
 
 int product_any(int type, const ProductP& p, bool wt, hipStream_t st) {
     return type == CT_F32 ? product_run<FF>(p, wt, st) : type == CT_BF16 ? product_run<BF>(p, wt, st) : product_run<HF>(p, wt, st);
 }
 int dw_any(int type, const DwP& p, hipStream_t st) { return type == CT_F32 ? dw_run<FF>(p, st) : type == CT_BF16 ? dw_run<BF>(p, st) : dw_run<HF>(p, st); }
+int grad_any(int type, const ProductP& x, const DwP& w, bool wt, hipStream_t st) {
+    return type == CT_F32 ? grad_run<FF>(x, w, wt, st) : type == CT_BF16 ? grad_run<BF>(x, w, wt, st) : grad_run<HF>(x, w, wt, st);
+}
 
 }  // namespace
 
@@ -626,7 +801,7 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
     if (rows == 0) return CT_OK;
     if (!offsets || !y || !x || !w || ldy < N || ldx < K || ldw < (w_transposed ? K : N) || w_group_stride < 0 || affine_stride < 0) return CT_EINVAL;
     if (ldx > kMaxStride || ldw > kMaxStride) return CT_ESHAPE;
-    const ProductP p{x, ldx, rows, K, w, w_group_stride, ldw, N, offsets, G, scale, shift, affine_stride, slope, fill_tail != 0, out_type == CT_F32, y, ldy, 0, 0, 0};
+    const ProductP p{x, ldx, rows, K, w, w_group_stride, ldw, N, offsets, G, scale, shift, affine_stride, slope, fill_tail != 0, out_type == CT_F32, y, ldy, 0, 0, 0, 0};
     return product_any(type, p, w_transposed != 0, (hipStream_t)stream);
 }
 
@@ -640,12 +815,11 @@ int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy
     if (dx && ((rows > 0 && !w) || ldw < (w_transposed ? K : N) || w_group_stride < 0 || lddx < K)) return CT_EINVAL;
     if (lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
     hipStream_t st = (hipStream_t)stream;
-    int rc = CT_OK;
-    if (dw) rc = dw_any(type, DwP{x, ldx, rows, K, dy, lddy, N, offsets, G, dw, dw_group_stride, lddw, out_type == CT_F32, 0, 0, 0}, st);
-    if (rc == CT_OK && dx && rows > 0)
-        rc = product_any(type, ProductP{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0},
-                         !w_transposed, st);
-    return rc;
+    const ProductP px{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0, 0};
+    const DwP pw{x, ldx, rows, K, dy, lddy, N, offsets, G, dw, dw_group_stride, lddw, out_type == CT_F32, 0, 0, 0};
+    if (dx && dw && rows > 0) return grad_any(type, px, pw, !w_transposed, st);
+    if (dx && rows > 0) return product_any(type, px, !w_transposed, st);
+    return dw ? dw_any(type, pw, st) : CT_OK;
 }
 
 }  // extern "C"

@@ -322,7 +322,7 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
  *     dx[r][k] = sum_n dy[r][n] w[g][k][n]                           [rows][K] of `type`, row stride lddx; zero behind offsets[G]
  *     dw[g][k][n] = sum over the rows r of group g of x[r][k] dy[r][n]    [G][K][N] of `out_type`; zero for a group without rows
  * x, w as above (w_transposed: stored [G][N][K]); dx or dw may be NULL (then w or x is not looked at).  dw: row stride lddw, group stride
- * dw_group_stride (groups must not overlap).  The order of every sum depends on the sizes alone.                                          */
+ * dw_group_stride (groups must not overlap).  The order of every sum depends on the sizes and on which of the two are asked for.         */
 size_t ct_grouped_product_grad_workspace_bytes(int type, int rows, int K, int N, int G);
 int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy, const void* x, int64_t ldx, int rows, int K, const void* w,
                             int64_t w_group_stride, int64_t ldw, int w_transposed, int N, const int32_t* offsets, int G, void* dx, int64_t lddx,
