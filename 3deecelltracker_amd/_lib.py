@@ -112,8 +112,7 @@ SIGNATURES = {
     "ct_correction_legacy_workspace_bytes": (_sz, [_ip, _i]),
     "ct_accurate_correction_legacy": (_i, [_vp, _vp, _i, _ip, _i, _i, _d, _i, _vp, _vp, _vp, _ip, _vp, _vp, _vp, _vp, _i, _ip, _vp, _sz, _vp]),
     "ct_trim_mean": (_i, [_vp, _i, _i, _d, _vp, _vp]),
-    "ct_grouped_product_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
-    "ct_grouped_product": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _i64, _f, _i, _vp, _i64, _vp, _sz, _vp]),
+    "ct_grouped_product": (_i, [_i, _i, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _i64, _f, _i, _vp, _i64, _vp]),
     "ct_grouped_product_grad_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "ct_grouped_product_grad": (_i, [_i, _i, _vp, _i64, _vp, _i64, _i, _i, _vp, _i64, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i64, _vp, _sz, _vp]),
     "ct_gradset_table_bytes": (_sz, [_i]),

@@ -15,33 +15,54 @@ namespace {
 constexpr int kChunk = 4096, kBlocks = 2048, kThreads = 256;
 
 struct Entry { const void* in; void* out; int64_t n; int64_t first; int64_t type; };     // first: chunks of the tensors before it
-constexpr int kPerLaunch = 64;
+constexpr int kWords = sizeof(Entry) / 8, kPerLaunch = 64;
 struct Batch { Entry e[kPerLaunch]; };                                                   // 2.5 KB of kernel arguments: the host's arrays are free on return
 
 __global__ __launch_bounds__(kPerLaunch) void table_kernel(const Batch b, int n, Entry* __restrict__ table) {
     if ((int)threadIdx.x < n) table[threadIdx.x] = b.e[threadIdx.x];
 }
 
-// table words are read with agent-scope loads: an earlier launch wrote them, and they stand at wave-uniform addresses (ct_fresh.h)
+// table words are read with agent-scope loads by lanes: an earlier launch wrote them, and plain loads of wave-uniform words would be scalar (ct_fresh.h)
 __device__ __forceinline__ int64_t word(const Entry* t, int i, int k) {
     return __hip_atomic_load(reinterpret_cast<const int64_t*>(t + i) + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 
 template <typename S> struct Piece { static constexpr int V = 16 / sizeof(S); S v[V]; };
 
-// f(entry, begin, end) for every run of values [begin, end) that this workgroup has
-template <typename F>
-__device__ __forceinline__ void each_run(const Entry* __restrict__ table, int n, F f) {
-    const int64_t total = word(table, n, 3);
+// The last entry that begins at or before chunk c (entries without values are passed over): the 64 lanes look at 64 entries at a time, so a list of
+// 1200 takes two loads after one another where halving would take eleven
+__device__ __forceinline__ int entry_of(const Entry* __restrict__ table, int n, int64_t c) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, span = n;
+    while (span > 1) {
+        const int step = (span + 63) / 64;
+        const bool in = lane * step < span;
+        const int k = __popcll(__ballot(in && word(table, in ? lo + lane * step : lo, 3) <= c)) - 1;
+        lo += k * step;
+        span = span - k * step < step ? span - k * step : step;
+    }
+    return lo;
+}
+
+// f(in, out, type, begin, end) for every run of values [begin, end) of one tensor that this workgroup has, in order or from the last to the first
+template <bool BACK, typename F>
+__device__ __forceinline__ void each_run(const Entry* __restrict__ table, int n, int64_t total, F f) {
     const int64_t c0 = total * blockIdx.x / gridDim.x, c1 = total * (blockIdx.x + 1) / gridDim.x;
     if (c0 >= c1) return;
-    int lo = 0, hi = n;                                     // the last entry that begins at or before c0: entries without values are passed over
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (word(table, mid, 3) <= c0) lo = mid; else hi = mid; }
-    for (int i = lo; i < n; ++i) {
-        const int64_t first = word(table, i, 3);
-        if (first >= c1) break;
-        const int64_t size = word(table, i, 2), b = (c0 > first ? c0 - first : 0) * kChunk, e = (c1 - first) * kChunk;
-        f(i, b, e < size ? e : size);
+    const int lane = threadIdx.x & 63;
+    int i = entry_of(table, n, BACK ? c1 - 1 : c0);
+    int64_t next = word(table, i, lane < kWords ? lane : 0);
+    for (; BACK ? i >= 0 : i < n; i += BACK ? -1 : 1) {
+        const int64_t e = next;
+        if (BACK ? i > 0 : i + 1 < n) next = word(table, i + (BACK ? -1 : 1), lane < kWords ? lane : 0);       // on its way while this tensor is read
+        const int64_t size = lane_of(e, 2), first = lane_of(e, 3);
+        if (!BACK && first >= c1) break;
+        const int64_t b = (c0 > first ? c0 - first : 0) * kChunk, end = (c1 - first) * kChunk;
+        if (b < (end < size ? end : size)) f((const void*)lane_of(e, 0), (void*)lane_of(e, 1), (int)lane_of(e, 4), b, end < size ? end : size);
+        if (BACK && first <= c0) break;
     }
 }
 
@@ -73,22 +94,26 @@ __device__ __forceinline__ double squares(const S* __restrict__ p, int64_t n) {
 #pragma unroll
             for (int k = 0; k < V; ++k) { const double x = (float)r[u].v[k]; acc = fma(x, x, acc); }
     }
-    for (; i < whole; i += kThreads) {
-        P r;
-        __builtin_memcpy(&r, p + i * V, 16);
-#pragma unroll
-        for (int k = 0; k < V; ++k) { const double x = (float)r.v[k]; acc = fma(x, x, acc); }
-    }
+    // the rest, its loads together: pieces that do not exist are the last one, and not counted
     const int64_t last = whole * V + threadIdx.x;
-    if (last < n) { const double x = (float)p[last]; acc = fma(x, x, acc); }
-    return acc;
+    const double x = last < n ? (double)(float)p[last] : 0.0;
+    if (whole > 0) {
+        P r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u], p + (i + u * kThreads < whole ? i + u * kThreads : whole - 1) * V, 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * kThreads < whole) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) { const double y = (float)r[u].v[k]; acc = fma(y, y, acc); }
+            }
+    }
+    return fma(x, x, acc);
 }
 
-__global__ __launch_bounds__(kThreads) void norm_kernel(const Entry* __restrict__ table, int n, double* __restrict__ part) {
+__global__ __launch_bounds__(kThreads) void norm_kernel(const Entry* __restrict__ table, int n, int64_t chunks, double* __restrict__ part) {
     double acc = 0.0;
-    each_run(table, n, [&](int i, int64_t b, int64_t e) {
-        const void* in = (const void*)word(table, i, 0);
-        const int type = (int)word(table, i, 4);
+    each_run<false>(table, n, chunks, [&](const void* in, void*, int type, int64_t b, int64_t e) {
         if (type == CT_F32) acc += squares((const float*)in + b, e - b);
         else if (type == CT_BF16) acc += squares((const __bf16*)in + b, e - b);
         else acc += squares((const _Float16*)in + b, e - b);
@@ -98,8 +123,14 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const Entry* __restrict_
 }
 
 __device__ __forceinline__ double norm_of(const double* __restrict__ part, int parts) {
-    double v = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kThreads) v += __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    double r[kBlocks / kThreads], v = 0.0;
+#pragma unroll
+    for (int u = 0; u < kBlocks / kThreads; ++u) {
+        const int i = threadIdx.x + u * kThreads;
+        r[u] = i < parts ? __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    }
+#pragma unroll
+    for (int u = 0; u < kBlocks / kThreads; ++u) v += r[u];
     return sqrt(block_sum(v));
 }
 
@@ -112,31 +143,36 @@ template <typename S>
 __device__ __forceinline__ void scaled(const S* p, S* o, int64_t n, float f, float f2) {
     typedef Piece<S> P;
     constexpr int V = P::V, U = 4;
-    const int64_t whole = n / V;
-    int64_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < whole; i += U * kThreads) {
+    const int64_t whole = n / V, last = whole * V + threadIdx.x;
+    const float x = last < n ? (float)p[last] : 0.f;
+    int64_t i = whole - 1 - threadIdx.x;
+    for (; i - (U - 1) * kThreads >= 0; i -= U * kThreads) {
         P r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u], p + (i + u * kThreads) * V, 16);
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u], p + (i - u * kThreads) * V, 16);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int k = 0; k < V; ++k) r[u].v[k] = (S)((float)r[u].v[k] * f * f2);
-            __builtin_memcpy(o + (i + u * kThreads) * V, &r[u], 16);
+            __builtin_memcpy(o + (i - u * kThreads) * V, &r[u], 16);
         }
     }
-    for (; i < whole; i += kThreads) {
-        P r;
-        __builtin_memcpy(&r, p + i * V, 16);
+    if (whole > 0) {                                        // the rest, its loads together
+        P r[U];
 #pragma unroll
-        for (int k = 0; k < V; ++k) r.v[k] = (S)((float)r.v[k] * f * f2);
-        __builtin_memcpy(o + i * V, &r, 16);
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r[u], p + (i - u * kThreads >= 0 ? i - u * kThreads : 0) * V, 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i - u * kThreads >= 0) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) r[u].v[k] = (S)((float)r[u].v[k] * f * f2);
+                __builtin_memcpy(o + (i - u * kThreads) * V, &r[u], 16);
+            }
     }
-    const int64_t last = whole * V + threadIdx.x;
-    if (last < n) o[last] = (S)((float)p[last] * f * f2);
+    if (last < n) o[last] = (S)(x * f * f2);
 }
 
-__global__ __launch_bounds__(kThreads) void clip_kernel(const Entry* __restrict__ table, int n, const double* __restrict__ part, int parts,
+__global__ __launch_bounds__(kThreads) void clip_kernel(const Entry* __restrict__ table, int n, int64_t chunks, const double* __restrict__ part, int parts,
                                                         double clip, float* __restrict__ norm_out) {
     const double norm = norm_of(part, parts);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
@@ -144,10 +180,8 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(const Entry* __restrict_
     // a factor below the 32-bit normal numbers is applied in two steps, the second a power of two
     const bool tiny = factor < 0x1p-100;
     const float f = (float)(tiny ? factor * 0x1p100 : factor), f2 = tiny ? 0x1p-100f : 1.f;
-    each_run(table, n, [&](int i, int64_t b, int64_t e) {
-        const void* in = (const void*)word(table, i, 0);
-        void* out = (void*)word(table, i, 1);
-        const int type = (int)word(table, i, 4);
+    // from the last values to the first: what the norm read last is still in the memory-side cache
+    each_run<true>(table, n, chunks, [&](const void* in, void* out, int type, int64_t b, int64_t e) {
         if (factor == 1.0 && in == out) return;
         if (type == CT_F32) scaled((const float*)in + b, (float*)out + b, e - b, f, f2);
         else if (type == CT_BF16) scaled((const __bf16*)in + b, (__bf16*)out + b, e - b, f, f2);
@@ -156,7 +190,11 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(const Entry* __restrict_
 }
 
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
-int blocks_of(int64_t chunks) { return chunks < 1 ? 1 : chunks < kBlocks ? (int)chunks : kBlocks; }
+// a workgroup a chunk up to 1024, then 4 chunks each: every workgroup of the second launch adds up the partial sums of all
+int blocks_of(int64_t chunks) {
+    const int64_t b = chunks <= 1024 ? chunks : chunks / 4 > 1024 ? chunks / 4 : 1024;
+    return b < 1 ? 1 : b < kBlocks ? (int)b : kBlocks;
+}
 
 }  // namespace
 
@@ -203,7 +241,7 @@ int ct_gradset_norm(const void* table, int n, int64_t chunks, float* norm, void*
     if (workspace_bytes < ct_gradset_workspace_bytes()) return CT_EWORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const int parts = blocks_of(chunks);
-    hipLaunchKernelGGL(norm_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, (double*)workspace);
+    hipLaunchKernelGGL(norm_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, chunks, (double*)workspace);
     hipLaunchKernelGGL(norm_only_kernel, dim3(1), dim3(kThreads), 0, st, (const double*)workspace, parts, norm);
     return (int)hipGetLastError();
 }
@@ -213,8 +251,8 @@ int ct_gradset_clip(const void* table, int n, int64_t chunks, double clip_norm, 
     if (workspace_bytes < ct_gradset_workspace_bytes()) return CT_EWORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const int parts = blocks_of(chunks);
-    hipLaunchKernelGGL(norm_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, (double*)workspace);
-    hipLaunchKernelGGL(clip_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, (const double*)workspace, parts, clip_norm, norm);
+    hipLaunchKernelGGL(norm_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, chunks, (double*)workspace);
+    hipLaunchKernelGGL(clip_kernel, dim3(parts), dim3(kThreads), 0, st, (const Entry*)table, n, chunks, (const double*)workspace, parts, clip_norm, norm);
     return (int)hipGetLastError();
 }
 

@@ -234,11 +234,6 @@ __device__ __forceinline__ f32x4 mfma(BF, s16x8 a, s16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma(HF, s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mfma(FF, f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-}
 
 // The bits of a fragment's contraction steps k0, k0 + 1, .. that lie in [lo, hi): whatever stands in the others, a NaN too, becomes zero
 template <bool H> __device__ __forceinline__ u32x4 steps_in(int k0, int lo, int hi) {
@@ -304,10 +299,19 @@ struct Core {
                 fb[i] = rb.read(stage + TA::BYTES, i, s0);
                 if (MASK) fb[i] = masked(fb[i], mask);
             }
+            if constexpr (H) {
 #pragma unroll
-            for (int i = 0; i < SN; ++i)
+                for (int i = 0; i < SN; ++i)
 #pragma unroll
-                for (int j = 0; j < SM; ++j) acc[i][j] = mfma(TT{}, fb[i], fa[j], acc[i][j]);
+                    for (int j = 0; j < SM; ++j) acc[i][j] = mfma(TT{}, fb[i], fa[j], acc[i][j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)                             // (the four of one strip depend on each other: the other strips' stand between them)
+#pragma unroll
+                    for (int i = 0; i < SN; ++i)
+#pragma unroll
+                        for (int j = 0; j < SM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[i][k], fa[j][k], acc[i][j], 0, 0, 0);
+            }
         }
     }
 
@@ -574,6 +578,7 @@ struct DwP {
     const void* dy; int64_t lddy; int N;
     const int32_t* off; int G;
     void* dw; int64_t wg, ldw;
+    float* part; int step, slots;            // a long sum in parts of `step` rows, [slot][K][N] (part NULL: no parts)
     int out32, mt, nt, count;
 };
 
@@ -584,14 +589,57 @@ __device__ __forceinline__ void dw_tile(const DwP& p, int id, unsigned char* sme
     constexpr int BM = Sh::BM, BN = Sh::BN;
     const int tile = tile_number(id, p.count), g = tile / (p.mt * p.nt), t = tile - g * p.mt * p.nt;
     const int nom_m = (t / p.nt) * BM, m0 = moved_back(nom_m, BM, p.K), nom_n = (t % p.nt) * BN, n0 = moved_back(nom_n, BN, p.N);
-    const int b = clampi(fresh_i32(p.off + g), 0, p.rows), e = clampi(fresh_i32(p.off + g + 1), b, p.rows);
+    int b, e;
+    if (p.part) {                            // g is a part's number
+        const Slot s = find_slot(p.off, p.G, p.rows, p.step, g, false);
+        if (s.group < 0) return;
+        b = s.row; e = s.end - s.row < p.step ? s.end : s.row + p.step;
+    } else {
+        b = clampi(fresh_i32(p.off + g), 0, p.rows); e = clampi(fresh_i32(p.off + g + 1), b, p.rows);
+    }
     C core;
     core.template run<false>(smem, (const S*)p.x + m0, (uint32_t)p.ldx, p.K - m0, p.K, 1, [&](int) { return (const S*)p.dy + n0; }, (uint32_t)p.lddy, [&](int) { return p.N - n0; }, p.N, b, e,
              p.rows, [](int) {});
+    if (p.part) {
+        float* const part = p.part + ((int64_t)g * p.K + m0) * p.N + n0;
+        core.each([](int) {}, [&](int m, int n, f32x4 v) {
+            if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store4(part + (int64_t)m * p.N + n, v, nom_n - n0 - n, p.N - n0 - n);
+        });
+        return;
+    }
     const int64_t at = g * p.wg + m0 * p.ldw + n0;
     core.each([](int) {}, [&](int m, int n, f32x4 v) {
         if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store_out<S>(p.dw, at + m * p.ldw + n, p.out32, v, nom_n - n0 - n, p.N - n0 - n);
     });
+}
+
+// Parts before group g, and its own
+__device__ __forceinline__ int2 parts_of(const int32_t* __restrict__ off, int rows, int step, int g) {
+    const int lane = threadIdx.x & 63;
+    int before = 0, own = 0;
+    for (int h = lane; h <= g; h += 64) {
+        const int b = clampi(off[h], 0, rows), n = (clampi(off[h + 1], b, rows) - b + step - 1) / step;
+        if (h < g) before += n; else own = n;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) { before += __shfl_xor(before, d); own += __shfl_xor(own, d); }
+    return int2{before, own};
+}
+// dw[g] = the sum of its parts, in order
+template <typename S>
+__global__ __launch_bounds__(256) void join_kernel(const DwP p) {
+    const int per = (p.K * p.N + 255) / 256, g = blockIdx.x / per;
+    const int2 at = parts_of(p.off, p.rows, p.step, g);
+    const int i = (blockIdx.x - g * per) * 256 + threadIdx.x;
+    if (i >= p.K * p.N) return;
+    const float* q = p.part + (int64_t)at.x * p.K * p.N + i;
+    const int own = at.x + at.y <= p.slots ? at.y : p.slots - at.x;              // (offsets that do not rise can count more parts than there are)
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < own; ++s) v += q[(int64_t)s * p.K * p.N];
+    const int k = i / p.N;
+    const int64_t to = g * p.wg + k * p.ldw + (i - k * p.N);
+    if (p.out32) ((float*)p.dw)[to] = v; else ((S*)p.dw)[to] = (S)v;
 }
 
 template <typename TT, bool WT, typename Sh>
@@ -638,7 +686,7 @@ template <typename Sh>
 int plan(DwP& p) {
     if (Sh::WAY != EDGE && (p.rows < Sh::BK || p.K < Sh::BM || p.N < Sh::BN)) return CT_EINVAL;
     p.mt = (p.K + Sh::BM - 1) / Sh::BM; p.nt = (p.N + Sh::BN - 1) / Sh::BN;
-    const int64_t count = (int64_t)p.G * p.mt * p.nt;
+    const int64_t count = (int64_t)(p.part ? p.slots : p.G) * p.mt * p.nt;
     if (count > kMaxBlocks) return CT_ESHAPE;
     p.count = (int)count;
     return CT_OK;
@@ -720,13 +768,33 @@ int product_pick(const ProductP& p, hipStream_t st) {
     }
     return launch<TT, WT, Any>(p, st);
 }
+// Few tiles with long sums: rows a part (0: the sums stay whole).  2 x 512 x 61 weights from 2 x 1024 rows are 16 tiles of 64 x 64.
+int part_rows(int rows, int K, int N, int G) {
+    const int64_t blocks = G * tiles(K, N, 64, 64), mean = rows / G;
+    if (blocks >= 64 || mean < 512) return 0;
+    const int64_t want = (2 * kCus + blocks - 1) / blocks, step = ((mean + want - 1) / want + 63) / 64 * 64;
+    return (int)(step < 128 ? 128 : step);
+}
+int part_slots(int rows, int step, int G) { return rows / step + (rows < G ? rows : G); }
+
 template <typename TT, Way WAY>
 int dw_pick(const DwP& p, hipStream_t st) {
     const int r = p.rows, k = p.K, n = p.N;
+    if (p.part) {
+        int rc;
+        if (WAY != EDGE && sizeof(typename TT::S) == 2 && k >= 64 && n >= 64) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 2, T64<WAY>, Any>>(p, st);
+        else if (sizeof(typename TT::S) == 4 && k >= 32 && n >= 32) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 4, F32s, Any>>(p, st);
+        else rc = launch<TT, Any>(p, st);
+        if (rc != CT_OK) return rc;
+        hipLaunchKernelGGL((join_kernel<typename TT::S>), dim3((unsigned)(p.G * ((p.K * p.N + 255) / 256))), dim3(256), 0, st, p);
+        return (int)hipGetLastError();
+    }
     if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
         if constexpr (WAY == DIRECT)
             if (r >= 64 && k >= 256 && n >= 256 && p.G * tiles(k, n, 256, 256) >= kCus) return launch<TT, T256<WAY>>(p, st);
         if (r >= 64 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= 160) return launch<TT, T128<WAY>>(p, st);
+        if constexpr (WAY == DIRECT)
+            if (r >= 256 && k >= 64 && n >= 64 && p.G * tiles(k, n, 64, 64) < kCus) return launch<TT, T64deep>(p, st);
         if (r >= 64 && k >= 64 && n >= 64) return launch<TT, T64<WAY>>(p, st);
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
@@ -741,7 +809,7 @@ template <typename TT, bool WT, Way WAY>
 int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     const int64_t mean = (x.rows + x.G - 1) / x.G, r = x.rows + x.G * 32;
     auto sum = [&](int t) { return tiles(r, x.N, t, t) + w.G * tiles(w.K, w.N, t, t); };
-    const int least = w.K < w.N ? w.K : w.N;                // both widths bound a tile of dw
+    const int least = w.part ? 0 : w.K < w.N ? w.K : w.N;   // both widths bound a tile of dw
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2)
         if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return launch<TT, WT, T256<WAY>, T256<WAY>>(x, w, st);
     if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
@@ -752,7 +820,7 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
         if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
         if (mean > 16 && x.rows >= 64 && least >= 64) return sum(64) >= 2 * kCus ? launch<TT, WT, F64, F64>(x, w, st) : launch<TT, WT, F32, F32s>(x, w, st);
     }
-    const int rc = dw_pick<TT, WAY>(w, st);
+    const int rc = dw_pick<TT, WAY>(w, st);                 // (also a sum in parts)
     return rc == CT_OK ? product_pick<TT, WT, WAY>(x, st) : rc;
 }
 
@@ -792,11 +860,9 @@ int grad_any(int type, const ProductP& x, const DwP& w, bool wt, hipStream_t st)
 
 extern "C" {
 
-size_t ct_grouped_product_workspace_bytes(int type, int rows, int K, int N, int G) { return 0; }
-
 int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
                        int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
-                       float slope, int fill_tail, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, ct_stream_t stream) {
+                       float slope, int fill_tail, void* y, int64_t ldy, ct_stream_t stream) {
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0) return CT_EINVAL;
     if (rows == 0) return CT_OK;
     if (!offsets || !y || !x || !w || ldy < N || ldx < K || ldw < (w_transposed ? K : N) || w_group_stride < 0 || affine_stride < 0) return CT_EINVAL;
@@ -805,7 +871,11 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
     return product_any(type, p, w_transposed != 0, (hipStream_t)stream);
 }
 
-size_t ct_grouped_product_grad_workspace_bytes(int type, int rows, int K, int N, int G) { return 0; }
+size_t ct_grouped_product_grad_workspace_bytes(int type, int rows, int K, int N, int G) {
+    if (!type_ok(type) || rows <= 0 || K <= 0 || N <= 0 || G <= 0) return 0;
+    const int step = part_rows(rows, K, N, G);
+    return step ? (size_t)part_slots(rows, step, G) * K * N * sizeof(float) : 0;
+}
 
 int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy, const void* x, int64_t ldx, int rows, int K, const void* w,
                             int64_t w_group_stride, int64_t ldw, int w_transposed, int N, const int32_t* offsets, int G, void* dx, int64_t lddx,
@@ -816,7 +886,11 @@ int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy
     if (lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
     hipStream_t st = (hipStream_t)stream;
     const ProductP px{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0, 0};
-    const DwP pw{x, ldx, rows, K, dy, lddy, N, offsets, G, dw, dw_group_stride, lddw, out_type == CT_F32, 0, 0, 0};
+    const int step = dw && rows > 0 ? part_rows(rows, K, N, G) : 0;
+    if (step && (!workspace || ((uintptr_t)workspace & 3))) return CT_EINVAL;
+    if (step && workspace_bytes < ct_grouped_product_grad_workspace_bytes(type, rows, K, N, G)) return CT_EWORKSPACE;
+    const DwP pw{x, ldx, rows, K, dy, lddy, N, offsets, G, dw, dw_group_stride, lddw, step ? (float*)workspace : nullptr, step, step ? part_slots(rows, step, G) : 0,
+                 out_type == CT_F32, 0, 0, 0};
     if (dx && dw && rows > 0) return grad_any(type, px, pw, !w_transposed, st);
     if (dx && rows > 0) return product_any(type, px, !w_transposed, st);
     return dw ? dw_any(type, pw, st) : CT_OK;

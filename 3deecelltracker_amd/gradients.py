@@ -11,7 +11,7 @@ import ctypes as C
 import math
 
 from . import _dev, _lib
-from .grouped import _On, _env
+from .grouped import _env, _on_device
 
 
 def _dense(a):
@@ -93,31 +93,31 @@ class GradientSet:
         ins = (C.c_void_p * m)(*[g.data_ptr() for g in self.grads])
         outs = (C.c_void_p * m)(*[o.data_ptr() for o in self.out])
         self._chunks = L.ct_gradset_chunks(n, sizes)
-        with _On(t, self._device) as stream:
+        with t.cuda.device(self._device):
             self._table = _dev.workspace(L.ct_gradset_table_bytes(n), self._device)
-            _lib.check(L.ct_gradset_write(n, ins, outs, sizes, types, self._table.data_ptr(), self._table.numel(), stream), "ct_gradset_write")
-        self._ws = L.ct_gradset_workspace_bytes()
+            _lib.check(L.ct_gradset_write(n, ins, outs, sizes, types, self._table.data_ptr(), self._table.numel(), _dev.stream(self._device)),
+                       "ct_gradset_write")
+        self._ws, self._at = L.ct_gradset_workspace_bytes(), self._table.data_ptr()
 
-    def _call(self, name, *args):
-        t, _, L = _env()
+    def _call(self, call, *args):
+        t = _env()[0]
         # the scalar and the partial sums, new for each call: two streams, or two graphs, share none
         scalar, ws = t.empty((), dtype=t.float32, device=self._device), t.empty(self._ws, dtype=t.uint8, device=self._device)
-        with _On(t, self._device) as stream:
-            rc = getattr(L, name)(self._table.data_ptr(), self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws, stream)
+        rc = _on_device(t, self._device, call, self._at, self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws)
         if rc:
-            _lib.check(rc, name)
+            _lib.check(rc, call.__name__)
         return scalar
 
     def norm(self):
         """The l2 norm over all values, a float32 scalar on the device (asynchronous)."""
-        return self._call("ct_gradset_norm")
+        return self._call(_env()[2].ct_gradset_norm)
 
     def clip(self, clip_norm: float):
         """Scale the gradients to at most `clip_norm` (into `out`, or in place) -> their norm before that, a float32 scalar on the device."""
         clip_norm = float(clip_norm)
         if not (clip_norm > 0.0 and math.isfinite(clip_norm)):
             raise ValueError(f"clip_norm must be positive and finite, got {clip_norm}")
-        return self._call("ct_gradset_clip", clip_norm)
+        return self._call(_env()[2].ct_gradset_clip, clip_norm)
 
 
 def clip_by_global_norm(grads, clip_norm: float, out=None):

@@ -20,7 +20,8 @@ _ready = None
 
 
 def _env():
-    """(torch, {type: CT_F32 / CT_BF16 / CT_F16}, the library), looked up once: these calls are short enough for the look-ups to count"""
+    """(torch, {type: CT_F32 / CT_BF16 / CT_F16}, the library), looked up once.  The kernels of a small layer take less time than a dozen look-ups: the
+    calls below test everything they ask of their operands in one expression, and only where that fails find out what is wrong."""
     global _ready
     if _ready is None:
         t = _lib.require_gpu()
@@ -61,11 +62,11 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
     the device already (a router's counts, summed there) is taken as it is, since looking at it would wait for the stream."""
     t = _env()[0]
     if isinstance(offsets, t.Tensor) and offsets.is_cuda:
+        if offsets.device == device and offsets.dtype is t.int32 and offsets.shape == (groups + 1,) and offsets.is_contiguous():
+            return offsets
         if offsets.dtype is not t.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
             raise ValueError(f"offsets: expected a contiguous int32 tensor of {groups + 1} numbers, got {offsets.dtype} {tuple(offsets.shape)}")
-        if offsets.device != device:
-            raise ValueError(f"offsets: are on {offsets.device}, the other tensors are on {device}")
-        return offsets
+        raise ValueError(f"offsets: are on {offsets.device}, the other tensors are on {device}")
     host = [int(v) for v in (offsets.tolist() if hasattr(offsets, "tolist") else offsets)]
     if len(host) != groups + 1:
         raise ValueError(f"offsets: expected {groups + 1} numbers for {groups} groups, got {len(host)}")
@@ -109,21 +110,12 @@ def _overlap(a, b):
     return p < s and r < q
 
 
-class _On:
-    """The calls run on the calling thread's current device: make it the tensors' where it is another, and name its current stream"""
-
-    def __init__(self, t, device):
-        self._guard = t.cuda.device(device) if t.cuda.current_device() != device.index else None
-        self.stream = t._C._cuda_getCurrentRawStream(device.index)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *a):
-        if self._guard is not None:
-            self._guard.__exit__(*a)
+def _on_device(t, device, call, *args):
+    """call(*args, stream) with `device` current: entry points without a handle run on the calling thread's current device"""
+    if t._C._cuda_getDevice() == device.index:
+        return call(*args, t._C._cuda_getCurrentRawStream(device.index))
+    with t.cuda.device(device):
+        return call(*args, t._C._cuda_getCurrentRawStream(device.index))
 
 
 def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, slope: float = 1.0, out=None, out_dtype=None):
@@ -133,9 +125,11 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
     the host or as int32 on the device; scale, shift: float32 [N] or [G, N].  Sums are held in 32 bits and rounded once to `out_dtype`
     (x's type, or float32).  Rows behind offsets[G] are zero in a new result and stay as they were in a given `out` [rows, N].  -> [rows, N]"""
     t, types, L = _env()
-    _check_tensor(t, types, "x", x, 2, None, None)
-    xt, device = x.dtype, x.device
-    _check_tensor(t, types, "w", w, 3, xt, device)
+    xt, device = getattr(x, "dtype", None), getattr(x, "device", None)
+    if not (xt in types and isinstance(w, t.Tensor) and w.dtype is xt and w.device == device and x.is_cuda and x.dim() == 2 and w.dim() == 3 and
+            not x.requires_grad and not w.requires_grad):
+        _check_tensor(t, types, "x", x, 2, None, None)
+        _check_tensor(t, types, "w", w, 3, xt, device)
     rows, k = x.shape
     g, wk, n, flip, ldw, group_stride = _weights("w", w, transposed)
     if wk != k:
@@ -162,12 +156,8 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
         ldy = _row_stride("out", rows, n, *out.stride())
         if _overlap(out, x) or _overlap(out, w):
             raise ValueError("out: overlaps x or w")
-    with _On(t, device) as stream:
-        need = L.ct_grouped_product_workspace_bytes(types[xt], rows, k, n, g)
-        ws = _dev.workspace(need, device) if need else None
-        rc = L.ct_grouped_product(types[xt], types[dtype], x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n, off.data_ptr(), g,
-                                  sc.data_ptr() if sc is not None else None, sh.data_ptr() if sh is not None else None, stride, slope, fill,
-                                  out.data_ptr(), ldy, ws.data_ptr() if need else None, need, stream)
+    rc = _on_device(t, device, L.ct_grouped_product, types[xt], types[dtype], x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n,
+                    off.data_ptr(), g, sc if sc is None else sc.data_ptr(), sh if sh is None else sh.data_ptr(), stride, slope, fill, out.data_ptr(), ldy)
     if rc:
         _lib.check(rc, "ct_grouped_product")
     return out
@@ -178,13 +168,16 @@ def product_grad(dy, x, w, offsets, *, need_x: bool = True, need_w: bool = True,
     `out_dtype`: w's type, or float32); None in the place of one that is not needed.  Rows behind offsets[G] get a zero dx, a group without
     rows a zero dw[g].  Of a block that w.expand shares, each group's part comes separately: sum them."""
     t, types, L = _env()
-    _check_tensor(t, types, "x", x, 2, None, None)
-    xt, device = x.dtype, x.device
-    _check_tensor(t, types, "w", w, 3, xt, device)
-    _check_tensor(t, types, "dy", dy, 2, xt, device)
+    xt, device = getattr(x, "dtype", None), getattr(x, "device", None)
+    if not (xt in types and isinstance(w, t.Tensor) and isinstance(dy, t.Tensor) and w.dtype is xt and dy.dtype is xt and w.device == device and
+            dy.device == device and x.is_cuda and x.dim() == 2 and w.dim() == 3 and dy.dim() == 2 and
+            not x.requires_grad and not w.requires_grad and not dy.requires_grad):
+        _check_tensor(t, types, "x", x, 2, None, None)
+        _check_tensor(t, types, "w", w, 3, xt, device)
+        _check_tensor(t, types, "dy", dy, 2, xt, device)
     rows, k = x.shape
     g, wk, n, flip, ldw, group_stride = _weights("w", w, False)
-    if wk != k or tuple(dy.shape) != (rows, n):
+    if wk != k or dy.shape != (rows, n):
         raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and w {tuple(w.shape)} do not fit each other")
     ldx, lddy = _row_stride("x", rows, k, *x.stride()), _row_stride("dy", rows, n, *dy.stride())
     dtype = out_dtype or xt
@@ -192,13 +185,15 @@ def product_grad(dy, x, w, offsets, *, need_x: bool = True, need_w: bool = True,
         raise ValueError(f"out_dtype: {dtype} is neither {xt} nor float32")
     off = offsets_device(offsets, g, rows, device)
     dx = t.empty((rows, k), dtype=xt, device=device) if need_x else None
-    dw = t.empty((g, k, n), dtype=dtype, device=device) if need_w else None
-    with _On(t, device) as stream:
+    dw, ws, need = None, None, 0
+    if need_w:
+        dw = t.empty((g, k, n), dtype=dtype, device=device)
         need = L.ct_grouped_product_grad_workspace_bytes(types[xt], rows, k, n, g)
-        ws = _dev.workspace(need, device) if need else None
-        rc = L.ct_grouped_product_grad(types[xt], types[dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n,
-                                       off.data_ptr(), g, dx.data_ptr() if need_x else None, k, dw.data_ptr() if need_w else None, k * n, n,
-                                       ws.data_ptr() if need else None, need, stream)
+        if need:
+            ws = _dev.workspace(need, device)
+    rc = _on_device(t, device, L.ct_grouped_product_grad, types[xt], types[dtype], dy.data_ptr(), lddy, x.data_ptr(), ldx, rows, k, w.data_ptr(),
+                    group_stride, ldw, flip, n, off.data_ptr(), g, dx.data_ptr() if need_x else None, k, dw.data_ptr() if need_w else None, k * n, n,
+                    ws.data_ptr() if need else None, need)
     if rc:
         _lib.check(rc, "ct_grouped_product_grad")
     return dx, dw

@@ -311,18 +311,18 @@ int ct_trim_mean(const double* stack, int k, int n3, double cut, double* out, ct
  * offsets [dev] int32 [G + 1], rising from 0 (offsets that do not are clamped: no access outside the tensors, but rows without a defined value).
  * scale, shift [dev] fp32 [G][N] with group stride affine_stride (0: one row for all groups), either may be NULL; slope 1: no activation.
  * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap x or w.  Sums are 32-bit, fp32
- * products exact; their order depends on the sizes alone.  Workspace: ct_grouped_product_workspace_bytes (may be 0: then NULL is fine).
- * CT_ESHAPE: a row stride above 2^22 values, or more than 2^22 tiles (of at least 16 x 32 values).                                                                                                           */
-size_t ct_grouped_product_workspace_bytes(int type, int rows, int K, int N, int G);
+ * products exact; their order depends on the sizes alone.
+ * CT_ESHAPE: a row stride above 2^22 values, or more than 2^22 tiles (of at least 16 x 32 values).                                          */
 int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
                        int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
-                       float slope, int fill_tail, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, ct_stream_t stream);
+                       float slope, int fill_tail, void* y, int64_t ldy, ct_stream_t stream);
 
 /* The gradients of ct_grouped_product (without scale, shift, act) for dy [dev] `type` [rows][N], row stride lddy:
  *     dx[r][k] = sum_n dy[r][n] w[g][k][n]                           [rows][K] of `type`, row stride lddx; zero behind offsets[G]
  *     dw[g][k][n] = sum over the rows r of group g of x[r][k] dy[r][n]    [G][K][N] of `out_type`; zero for a group without rows
  * x, w as above (w_transposed: stored [G][N][K]); dx or dw may be NULL (then w or x is not looked at).  dw: row stride lddw, group stride
- * dw_group_stride (groups must not overlap).  The order of every sum depends on the sizes and on which of the two are asked for.         */
+ * dw_group_stride (groups must not overlap).  The order of every sum depends on the sizes and on which of the two are asked for.
+ * Workspace [dev], 4-byte aligned: long sums for few weights are made in parts (0 bytes: NULL is fine).                                  */
 size_t ct_grouped_product_grad_workspace_bytes(int type, int rows, int K, int N, int G);
 int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy, const void* x, int64_t ldx, int rows, int K, const void* w,
                             int64_t w_group_stride, int64_t ldw, int w_transposed, int N, const int32_t* offsets, int G, void* dx, int64_t lddx,

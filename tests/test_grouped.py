@@ -70,6 +70,8 @@ CASES = [
     # the large tiles: more of them than compute units, partial in every direction
     ([4000, 0, 3500, 777], 72, 2050, 3), ([2100, 1, 2300], 136, 1161, 0), ([0, 90, 64, 131, 77, 1, 200, 63, 65, 2], 1300, 1290, 1),
     ([33, 0, 100, 5] * 4, 520, 517, 2), ([9] * 20 + [0] * 10 + [31], 700, 264, 2), ([40, 31], 2050, 70, 0),
+    # long sums for few weights
+    ([2300, 0, 1501], 61, 70, 3), ([1024, 1024], 61, 512, 0), ([5000], 128, 64, 1), ([1600, 3], 7, 33, 0),
 ]
 
 
@@ -298,7 +300,7 @@ def test_the_abi_refuses_without_a_gpu():
         importlib.import_module("__graft_entry__").build()
     L = _lib.lib()
     ok = dict(type=0, out=0, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, sc=None, sh=None, ag=0, slope=1.0, fill=1, y=64, ldy=6,
-              ws=None, wsb=0, st=None)
+              st=None)
     call = lambda **kw: L.ct_grouped_product(*{**ok, **kw}.values())
     for kw in (dict(type=3), dict(type=-1), dict(out=1), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(w=None), dict(off=None), dict(y=None),
                dict(ldx=7), dict(ldw=5), dict(ldy=5), dict(wg=-1), dict(ag=-1), dict(wt=1, ldw=7)):
@@ -311,5 +313,7 @@ def test_the_abi_refuses_without_a_gpu():
     for kw in (dict(type=3), dict(out=2), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(dy=None), dict(w=None), dict(off=None), dict(ldx=7),
                dict(lddy=5), dict(ldw=5), dict(lddw=5), dict(dwg=47), dict(lddx=7), dict(wg=-1), dict(wt=1, ldw=7)):
         assert call2(**kw) == _lib.CT_EINVAL, kw
+    assert L.ct_grouped_product_grad_workspace_bytes(0, 4, 8, 6, 2) == 0 and L.ct_grouped_product_grad_workspace_bytes(0, 2048, 8, 6, 2) > 0
+    assert call2(rows=2048) == _lib.CT_EINVAL and call2(rows=2048, ws=64, wsb=8) == _lib.CT_EWORKSPACE
     for kw in (dict(ldx=2 ** 22 + 1), dict(lddy=2 ** 22 + 1), dict(ldw=2 ** 22 + 1)):
         assert call2(**kw) == _lib.CT_ESHAPE, kw
