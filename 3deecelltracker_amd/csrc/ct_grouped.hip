@@ -726,13 +726,16 @@ template <Way W> using T64 = Shape<64, 64, 64, 2, 2, 1, 2, W>;
 using T64deep = Shape<64, 64, 64, 2, 2, 1, 4, DIRECT>;
 template <Way W> using T64flat = Shape<64, 64, 32, 2, 2, 1, 2, W>;
 using T32 = Shape<32, 64, 128, 1, 2, 2, 2, DIRECT>;
-using T16 = Shape<16, 64, 256, 1, 1, 4, 2, DIRECT>;
+using T32k = Shape<32, 32, 256, 1, 1, 8, 3, DIRECT>;
+using T32s = Shape<32, 32, 128, 1, 1, 4, 3, DIRECT>;
+using T16 = Shape<16, 64, 128, 1, 1, 4, 4, DIRECT>;
 using T16r = Shape<16, 64, 128, 1, 1, 4, 2, REGS>;
 using F128 = Shape<128, 128, 32, 2, 4, 1, 2, DIRECT>;
 using F64 = Shape<64, 64, 32, 2, 2, 1, 2, DIRECT>;
 using F32 = Shape<32, 64, 64, 1, 1, 4, 2, DIRECT>;
 using F32s = Shape<32, 32, 64, 1, 1, 4, 2, DIRECT>;
 using F16 = Shape<16, 64, 128, 1, 1, 4, 2, DIRECT>;
+using F16k = Shape<16, 32, 128, 1, 1, 8, 3, DIRECT>;
 using Any = Shape<64, 64, 32, 2, 2, 1, 2, EDGE>;
 
 // Which tile.  16 x 64: a few rows a group, bound by the weights, every wave a quarter of the sum.  Large tiles where there are enough of them for all
@@ -743,7 +746,10 @@ int product_pick(const ProductP& p, hipStream_t st) {
     const int k = p.K, n = WT ? 1 << 30 : p.N;              // what the tile must not exceed: rows of w may be repeated, columns may not
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2) {
         const int64_t t128 = tiles(r, p.N, 128, 128), t64 = tiles(r, p.N, 64, 64);
-        if (mean <= 16 && k >= 256 && n >= 64) return launch<TT, WT, T16>(p, st);
+        const int64_t t32 = tiles(r, p.N, 32, 32);
+        if (k >= 512 && n >= 32 && t32 < 2 * kCus) return launch<TT, WT, T32k>(p, st);
+        if (k >= 128 && n >= 32 && t32 < 2 * kCus) return launch<TT, WT, T32s>(p, st);
+        if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, T16>(p, st);
         if (mean >= 192 && k >= 64 && p.N >= 256 && tiles(r, p.N, 256, 256) >= kCus) return launch<TT, WT, T256<DIRECT>>(p, st);
         if (mean >= 96 && k >= 64 && p.N >= 128 && t128 >= kCus) return k <= 128 && t128 >= 4 * kCus ? launch<TT, WT, T128run>(p, st) : launch<TT, WT, T128<DIRECT>>(p, st);
         if (mean >= 96 && k >= 256 && p.N >= 128 && t128 >= 160) return launch<TT, WT, T128deep>(p, st);
@@ -760,6 +766,7 @@ int product_pick(const ProductP& p, hipStream_t st) {
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
         const int64_t t64 = tiles(r, p.N, 64, 64);
+        if (k >= 128 && n >= 32 && tiles(p.rows + p.G * 32, p.N, 16, 32) < kCus) return launch<TT, WT, F16k>(p, st);
         if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, F16>(p, st);
         if (mean >= 96 && k >= 32 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 2 * kCus) return launch<TT, WT, F128>(p, st);
         if (k >= 64 && n >= 64 && t64 < 2 * kCus && t64 >= kCus) return launch<TT, WT, F32>(p, st);

@@ -36,11 +36,24 @@ class FFN:
     bias)+BN+LeakyReLU, Dense(512->1)+sigmoid -- evaluated by the HIP library."""
 
     def __init__(self, device: int | None = None):
-        self._handle = None
+        self._loaded = None            # the library's handle
+        self._stale = False            # the training weights are ahead of it
+        self._training = None
         self._device = device
         self._weights = None
 
+    @property
+    def _handle(self):
+        if self._stale:
+            self._stale = False
+            self._upload(self._training.weights())
+        return self._loaded
+
     def set_weights_dict(self, w: dict):
+        self._training, self._stale = None, False
+        return self._upload(w)
+
+    def _upload(self, w: dict):
         t = _lib.require_gpu()
         if self._device is None:
             self._device = t.cuda.current_device()
@@ -51,7 +64,7 @@ class FFN:
         self._free()
         h = C.c_void_p()
         _lib.check(L.ct_ffn_create(flat.ctypes.data, flat.size, self._device, C.byref(h)), "ct_ffn_create")
-        self._handle = h
+        self._loaded = h
         self._weights = w
         return self
 
@@ -72,7 +85,32 @@ class FFN:
         from .keras_h5 import read_ffn_h5
         return self.set_weights_dict(read_ffn_h5(path))
 
+    def compile(self, learning_rate: float = 1e-3, beta_1: float = 0.9, beta_2: float = 0.999, epsilon: float = 1e-7, global_clipnorm: float | None = None):
+        """Start training from the present weights: Adam, binary cross-entropy, all gradients clipped together by `global_clipnorm` (Keras' names and
+        defaults; the loop around it, reference ffn.py:56-222, is the caller's)."""
+        from .ffn_training import FFNTraining
+        self._require()
+        self._training = FFNTraining(self._weights, f"cuda:{self._device}", learning_rate, beta_1, beta_2, epsilon, global_clipnorm)
+
+    def train_on_batch(self, x, y) -> float:
+        """One update from x -- (P,122), or the two halves [ (P,61), (P,61) ] -- and labels y (P,) or (P,1) in [0, 1]; numpy or torch -> the loss
+        before it.  predict() and the matching calls use the new weights."""
+        t = _lib.require_gpu()
+        if self._training is None:
+            raise ValueError("FFN is not being trained: call compile() first")
+        if isinstance(x, (list, tuple)):
+            x = t.cat([_dev.to_dev(h, t.float32, f"cuda:{self._device}") for h in x], dim=1)
+        x = _dev.to_dev(x, t.float32, f"cuda:{self._device}")
+        y = _dev.to_dev(y, t.float32, f"cuda:{self._device}").reshape(-1)
+        if x.ndim != 2 or x.shape[1] != 2 * FFN_FEAT or x.shape[0] < 2 or y.shape[0] != x.shape[0]:
+            raise ValueError(f"expected at least two rows (P, {2 * FFN_FEAT}) and as many labels, got {tuple(x.shape)} and {tuple(y.shape)}")
+        with t.cuda.device(x.device):
+            loss = self._training.step(x, y)
+        self._stale = True
+        return float(loss)
+
     def save_weights(self, path):
+        self._handle                                                      # (training weights come back first)
         w = self._weights
         if w is None:
             raise ValueError("model has no weights")
@@ -121,9 +159,9 @@ class FFN:
     __call__ = predict
 
     def _free(self):
-        if self._handle is not None:
-            _lib.lib().ct_ffn_destroy(self._handle)
-            self._handle = None
+        if self._loaded is not None:
+            _lib.lib().ct_ffn_destroy(self._loaded)
+            self._loaded = None
 
     def __del__(self):
         try:
