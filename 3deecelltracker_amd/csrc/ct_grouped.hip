@@ -582,7 +582,7 @@ struct DwP {
     int out32, mt, nt, count;
 };
 
-template <typename TT, typename Sh>
+template <typename TT, typename Sh, bool PARTS>
 __device__ __forceinline__ void dw_tile(const DwP& p, int id, unsigned char* smem) {
     typedef typename TT::S S;
     typedef typename Sh::template Of<TT, false, false> C;
@@ -590,7 +590,7 @@ __device__ __forceinline__ void dw_tile(const DwP& p, int id, unsigned char* sme
     const int tile = tile_number(id, p.count), g = tile / (p.mt * p.nt), t = tile - g * p.mt * p.nt;
     const int nom_m = (t / p.nt) * BM, m0 = moved_back(nom_m, BM, p.K), nom_n = (t % p.nt) * BN, n0 = moved_back(nom_n, BN, p.N);
     int b, e;
-    if (p.part) {                            // g is a part's number
+    if constexpr (PARTS) {                   // g is a part's number
         const Slot s = find_slot(p.off, p.G, p.rows, p.step, g, false);
         if (s.group < 0) return;
         b = s.row; e = s.end - s.row < p.step ? s.end : s.row + p.step;
@@ -600,17 +600,17 @@ __device__ __forceinline__ void dw_tile(const DwP& p, int id, unsigned char* sme
     C core;
     core.template run<false>(smem, (const S*)p.x + m0, (uint32_t)p.ldx, p.K - m0, p.K, 1, [&](int) { return (const S*)p.dy + n0; }, (uint32_t)p.lddy, [&](int) { return p.N - n0; }, p.N, b, e,
              p.rows, [](int) {});
-    if (p.part) {
+    if constexpr (PARTS) {
         float* const part = p.part + ((int64_t)g * p.K + m0) * p.N + n0;
         core.each([](int) {}, [&](int m, int n, f32x4 v) {
             if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store4(part + (int64_t)m * p.N + n, v, nom_n - n0 - n, p.N - n0 - n);
         });
-        return;
+    } else {
+        const int64_t at = g * p.wg + m0 * p.ldw + n0;
+        core.each([](int) {}, [&](int m, int n, f32x4 v) {
+            if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store_out<S>(p.dw, at + m * p.ldw + n, p.out32, v, nom_n - n0 - n, p.N - n0 - n);
+        });
     }
-    const int64_t at = g * p.wg + m0 * p.ldw + n0;
-    core.each([](int) {}, [&](int m, int n, f32x4 v) {
-        if (m >= nom_m - m0 && m < p.K - m0 && n < p.N - n0) store_out<S>(p.dw, at + m * p.ldw + n, p.out32, v, nom_n - n0 - n, p.N - n0 - n);
-    });
 }
 
 // Parts before group g, and its own
@@ -647,10 +647,10 @@ __global__ __launch_bounds__(Sh::THREADS) void product_kernel(const ProductP p) 
     __shared__ __attribute__((aligned(1024))) unsigned char smem[Sh::template Of<TT, true, WT>::LDS_BYTES];
     product_tile<TT, WT, Sh>(p, blockIdx.x, smem);
 }
-template <typename TT, typename Sh>
+template <typename TT, typename Sh, bool PARTS>
 __global__ __launch_bounds__(Sh::THREADS) void dw_kernel(const DwP p) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[Sh::template Of<TT, false, false>::LDS_BYTES];
-    dw_tile<TT, Sh>(p, blockIdx.x, smem);
+    dw_tile<TT, Sh, PARTS>(p, blockIdx.x, smem);
 }
 // Both gradients in one launch: neither alone fills the card at the sizes of a network's layers, and one launch costs as much as a small product
 template <typename TT, bool WT, typename ShX, typename ShW>
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(ShX::THREADS) void grad_kernel(const ProductP x, co
     constexpr int LX = ShX::template Of<TT, true, WT>::LDS_BYTES, LW = ShW::template Of<TT, false, false>::LDS_BYTES;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[LX > LW ? LX : LW];
     const int id = blockIdx.x, ahead = w_first ? w.count : x.count;
-    if ((id < ahead) == (w_first != 0)) dw_tile<TT, ShW>(w, w_first ? id : id - ahead, smem);
+    if ((id < ahead) == (w_first != 0)) dw_tile<TT, ShW, false>(w, w_first ? id : id - ahead, smem);
     else product_tile<TT, WT, ShX>(x, w_first ? id - ahead : id, smem);
 }
 
@@ -698,11 +698,11 @@ int launch(ProductP p, hipStream_t st) {
     hipLaunchKernelGGL((product_kernel<TT, WT, Sh>), dim3((unsigned)p.count), dim3(Sh::THREADS), 0, st, p);
     return (int)hipGetLastError();
 }
-template <typename TT, typename Sh>
+template <typename TT, typename Sh, bool PARTS = false>
 int launch(DwP p, hipStream_t st) {
     const int rc = plan<Sh>(p);
     if (rc != CT_OK) return rc;
-    hipLaunchKernelGGL((dw_kernel<TT, Sh>), dim3((unsigned)p.count), dim3(Sh::THREADS), 0, st, p);
+    hipLaunchKernelGGL((dw_kernel<TT, Sh, PARTS>), dim3((unsigned)p.count), dim3(Sh::THREADS), 0, st, p);
     return (int)hipGetLastError();
 }
 template <typename TT, bool WT, typename ShX, typename ShW>
@@ -736,7 +736,10 @@ using F32 = Shape<32, 64, 64, 1, 1, 4, 2, DIRECT>;
 using F32s = Shape<32, 32, 64, 1, 1, 4, 2, DIRECT>;
 using F16 = Shape<16, 64, 128, 1, 1, 4, 2, DIRECT>;
 using F16k = Shape<16, 32, 128, 1, 1, 8, 3, DIRECT>;
+using R64k = Shape<64, 64, 128, 2, 2, 2, 2, REGS>;
+using R32k = Shape<32, 32, 256, 1, 1, 8, 2, REGS>;
 using Any = Shape<64, 64, 32, 2, 2, 1, 2, EDGE>;
+template <int BK> using AnyK = Shape<32, 32, BK, 1, 1, 8, 2, EDGE>;
 
 // Which tile.  16 x 64: a few rows a group, bound by the weights, every wave a quarter of the sum.  Large tiles where there are enough of them for all
 // CUs, since each value of an operand is then fetched less often; else small ones.
@@ -759,8 +762,10 @@ int product_pick(const ProductP& p, hipStream_t st) {
         if (k >= 32 && n >= 64) return launch<TT, WT, T64flat<DIRECT>>(p, st);
     }
     if constexpr (WAY == REGS && sizeof(typename TT::S) == 2) {
+        if (k >= 512 && n >= 32 && tiles(r, p.N, 32, 32) < 2 * kCus) return launch<TT, WT, R32k>(p, st);
         if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, T16r>(p, st);
         if (mean >= 96 && k >= 64 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 160) return launch<TT, WT, T128<REGS>>(p, st);
+        if (k >= 512 && n >= 64 && tiles(r, p.N, 64, 64) < kCus) return launch<TT, WT, R64k>(p, st);
         if (k >= 64 && n >= 64) return launch<TT, WT, T64<REGS>>(p, st);
         if (k >= 32 && n >= 64) return launch<TT, WT, T64flat<REGS>>(p, st);
     }
@@ -773,6 +778,8 @@ int product_pick(const ProductP& p, hipStream_t st) {
         if (k >= 64 && n >= 32 && t64 < kCus) return launch<TT, WT, F32s>(p, st);
         if (k >= 32 && n >= 64) return launch<TT, WT, F64>(p, st);
     }
+    // narrower than any tile above: long sums in wide stages over 8 waves
+    if (k >= 512 && tiles(r, p.N, 32, 32) < 2 * kCus) return launch<TT, WT, AnyK<1024 / (int)sizeof(typename TT::S)>>(p, st);
     return launch<TT, WT, Any>(p, st);
 }
 // Few tiles with long sums: rows a part (0: the sums stay whole).  2 x 512 x 61 weights from 2 x 1024 rows are 16 tiles of 64 x 64.
@@ -789,9 +796,9 @@ int dw_pick(const DwP& p, hipStream_t st) {
     const int r = p.rows, k = p.K, n = p.N;
     if (p.part) {
         int rc;
-        if (WAY != EDGE && sizeof(typename TT::S) == 2 && k >= 64 && n >= 64) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 2, T64<WAY>, Any>>(p, st);
-        else if (sizeof(typename TT::S) == 4 && k >= 32 && n >= 32) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 4, F32s, Any>>(p, st);
-        else rc = launch<TT, Any>(p, st);
+        if (WAY != EDGE && sizeof(typename TT::S) == 2 && k >= 64 && n >= 64) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 2, T64<WAY>, Any>, true>(p, st);
+        else if (sizeof(typename TT::S) == 4 && k >= 32 && n >= 32) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 4, F32s, Any>, true>(p, st);
+        else rc = launch<TT, Any, true>(p, st);
         if (rc != CT_OK) return rc;
         hipLaunchKernelGGL((join_kernel<typename TT::S>), dim3((unsigned)(p.G * ((p.K * p.N + 255) / 256))), dim3(256), 0, st, p);
         return (int)hipGetLastError();
@@ -825,7 +832,14 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
         if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
-        if (mean > 16 && x.rows >= 64 && least >= 64) return sum(64) >= 2 * kCus ? launch<TT, WT, F64, F64>(x, w, st) : launch<TT, WT, F32, F32s>(x, w, st);
+        if (mean > 16 && x.rows >= 64 && least >= 64) {
+            // 32 x 64 tiles (48 KB: 3 on a CU) where they all run at once and fill it: 2048 x 512 x 512 in 2 groups 23.3 us, 27.4 with 32 x 32;
+            // 500 x 200 x 1000 in 4 groups 16.9, 12.8 with 32 x 32
+            const int64_t n64 = tiles(r, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64);
+            if (sum(64) >= 2 * kCus && n64 > 4 * kCus) return launch<TT, WT, F64, F64>(x, w, st);
+            if (n64 >= 2 * kCus && n64 <= 3 * kCus + kCus / 8) return launch<TT, WT, F32, F32>(x, w, st);
+            return launch<TT, WT, F32s, F32s>(x, w, st);
+        }
     }
     const int rc = dw_pick<TT, WAY>(w, st);                 // (also a sum in parts)
     return rc == CT_OK ? product_pick<TT, WT, WAY>(x, st) : rc;

@@ -11,6 +11,7 @@ csrc/ct_match.hip.  The (m*n) x 122 pair grid the reference tiles on the host is
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from pathlib import Path
 from typing import Tuple, Union
 
@@ -39,14 +40,17 @@ class FFN:
         self._loaded = None            # the library's handle
         self._stale = False            # the training weights are ahead of it
         self._training = None
+        self._lock = threading.Lock()
         self._device = device
         self._weights = None
 
     @property
     def _handle(self):
         if self._stale:
-            self._stale = False
-            self._upload(self._training.weights())
+            with self._lock:                   # (matches run on several host threads: the first one brings the weights, the others wait)
+                if self._stale:
+                    self._upload(self._training.weights())
+                    self._stale = False
         return self._loaded
 
     def set_weights_dict(self, w: dict):

@@ -39,7 +39,7 @@ class FFNTraining:
         views = lambda buf: dict(zip(TRAINED, (p.view(first[k].shape) for k, p in zip(TRAINED, t.split(buf, [first[k].numel() for k in TRAINED])))))
         self.w, self.g = views(self.flat), views(self.grad)
         self.moving = {k: up(weights[b][n], hid).clone() for k, b, n in (("mean1", "bn1", "mean"), ("var1", "bn1", "var"), ("mean2", "bn2", "mean"), ("var2", "bn2", "var"))}
-        self.steps = 0
+        self.steps, self.offsets = 0, {}
 
     @staticmethod
     def _normalise(h, gamma, beta):
@@ -64,7 +64,9 @@ class FFNTraining:
         t = _dev.torch()
         rows, hid = x.shape[0], self.w["w3"].shape[1]
         halves = x.view(rows, 2, FFN_FEAT).transpose(0, 1).reshape(2 * rows, FFN_FEAT)
-        one, two, last = [0, 2 * rows], [0, rows, 2 * rows], [0, rows]
+        if rows not in self.offsets:                                  # one group of all rows, the two halves, the rows of the pairs
+            self.offsets = {rows: [t.tensor(o, dtype=t.int32).to(x.device) for o in ([0, 2 * rows], [0, rows, 2 * rows], [0, rows])]}
+        one, two, last = self.offsets[rows]
         h1, s1 = self._normalise(product(halves, self.w["w1"], one).view(2, rows, hid), self.w["gamma1"], self.w["beta1"])
         h1 = h1.view(2 * rows, hid)
         pair = product(h1, self.w["w2"], two).view(2, rows, hid)

@@ -72,6 +72,8 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
         raise ValueError(f"offsets: expected {groups + 1} numbers for {groups} groups, got {len(host)}")
     if host[0] != 0 or any(a > b for a, b in zip(host, host[1:])) or host[-1] > rows:
         raise ValueError(f"offsets: must rise from 0 to at most {rows} rows")
+    if t.cuda.is_current_stream_capturing():
+        raise ValueError("offsets: numbers on the host cannot be uploaded while a graph is captured; pass an int32 tensor on the device")
     return t.tensor(host, dtype=t.int32).to(device)
 
 

@@ -70,6 +70,8 @@ CASES = [
     # the large tiles: more of them than compute units, partial in every direction
     ([4000, 0, 3500, 777], 72, 2050, 3), ([2100, 1, 2300], 136, 1161, 0), ([0, 90, 64, 131, 77, 1, 200, 63, 65, 2], 1300, 1290, 1),
     ([33, 0, 100, 5] * 4, 520, 517, 2), ([9] * 20 + [0] * 10 + [31], 700, 264, 2), ([40, 31], 2050, 70, 0),
+    # long sums for few columns, of even and odd width
+    ([2, 0, 3], 3181, 16, 2), ([90, 1], 1024, 30, 0), ([100, 40], 1001, 333, 0), ([300, 41], 2755, 411, 1), ([33], 600, 1, 0),
     # long sums for few weights
     ([2300, 0, 1501], 61, 70, 3), ([1024, 1024], 61, 512, 0), ([5000], 128, 64, 1), ([1600, 3], 7, 33, 0),
 ]
@@ -207,6 +209,43 @@ def test_values_that_are_not_finite_stay_in_their_rows(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k,n", [(96, 80), (300, 260), (61, 40)])
+def test_values_that_are_not_finite_stay_in_their_group(dtype, k, n):
+    """A stage of the sum over a group's rows may begin in its neighbour's: what stands there does not count"""
+    t = _torch()
+    counts = [70, 1, 66, 0, 130, 7]
+    x, dy, w = _rand((280, k), dtype, 1), _rand((280, n), dtype, 2), _rand((6, k, n), dtype, 3)
+    off = _offsets(counts)
+    clean = grouped.product_grad(dy, x, w, off)
+    x[100, :] = float("nan"); dy[71:137] = float("inf"); x[274:] = float("nan"); dy[274:] = float("nan")       # group 2, and behind the last
+    dx, dw = grouped.product_grad(dy, x, w, off)
+    for g in (0, 1, 3, 4, 5):
+        assert t.equal(dw[g], clean[1][g]), g
+    assert not bool(t.isfinite(dw[2]).any()) and t.equal(dx[:71], clean[0][:71]) and t.equal(dx[137:274], clean[0][137:274])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_offsets_past_32_bits(dtype):
+    """Rows and weight blocks whose first value lies more than 2^31 values into the tensor"""
+    t = _torch()
+    x = t.zeros(70000, 40000, device="cuda", dtype=getattr(t, dtype))[:, :64]
+    w = t.zeros(3, 40000, 40000, device="cuda", dtype=getattr(t, dtype))[:, -64:, -96:] if dtype == "bfloat16" else _rand((3, 64, 96), dtype, 2)
+    x[-80:].copy_(_rand((80, 64), dtype, 1)); w[1:].copy_(_rand((2, 64, 96), dtype, 3, 0.1))
+    off = [0, 69000, 69930, 70000]
+    y = grouped.product(x, w, off)
+    want, bound = _ref(x[-80:], w[1:], [10, 70])
+    _check(y[-80:], want, bound, y.dtype)
+    dy = _rand((70000, 96), dtype, 4)
+    dx, dw = grouped.product_grad(dy, x, w, off)
+    want, bound = _ref(dy[-80:], w[1:].transpose(1, 2), [10, 70])
+    _check(dx[-80:], want, bound, dx.dtype)
+    xs, ds = x[-70:].double().cpu(), dy[-70:].double().cpu()
+    _check(dw[2], xs.T @ ds, (74 * UNIT) * (xs.abs().T @ ds.abs()), dw.dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_shared_block_equals_one_group(dtype):
     t = _torch()
     counts = [33, 0, 190, 64]
@@ -237,6 +276,8 @@ def test_offsets_on_the_device_and_streams_and_graphs():
     assert all(t.equal(v, y) for v in a) and all(t.equal(v, dx) and t.equal(u, dw) for v, u in b)
     graph = t.cuda.CUDAGraph()
     with t.cuda.graph(graph):
+        with pytest.raises(ValueError):
+            grouped.product(x, w, _offsets(counts))                      # numbers on the host cannot be uploaded here
         gy = grouped.product(x, w, dev_off); gx, gw = grouped.product_grad(dy, x, w, dev_off)
     for seed, c in ((11, counts), (12, [0, 0, 340, 0, 0]), (13, [68] * 5), (14, [1, 2, 3, 4, 5])):
         x.copy_(_rand((340, 128), "bfloat16", seed)); dev_off.copy_(t.tensor(_offsets(c), dtype=t.int32))
