@@ -8,6 +8,20 @@
 //   product           A = x   (c contiguous)   B = w   (n contiguous)
 //   product, w^T      A = dy  (c contiguous)   B = w   (c contiguous)
 //   dw                A = x   (m contiguous)   B = dy  (n contiguous), c = the group's rows
+//
+// What bounds it, and what was chosen for it (measured on MI355X; a copy runs at 5.1 TB/s there, a library product of 8192^3 at 1189 TFLOP/s in bf16
+// and 153 in fp32):
+//   * large groups, 16 bit: the matrix pipe (55 % busy) and, next to it, LDS.  256 x 256 tiles of 8 waves, two 64 KB stages filled by direct loads:
+//     32768 x 4096 x 2048 in 16 uneven groups 560 us = 980 TFLOP/s (542-575 over boxes; 128 x 128 tiles 650), its gradients at 16384 x 2048 x 1536 285 us.
+//   * a few rows a group: the weights, each read once.  16 x 64 tiles, every wave a quarter of a stage's sum: 64 rows of 2048 x 1024 blocks 32 us
+//     for the ~35 blocks that have rows, 42 us with all 64 (6.4 TB/s).
+//   * in between: bytes from L2 to LDS (about 9.5 TB/s) and the latency of a stage; what helped was more workgroups on a CU, so two stages rather than three
+//     or four wherever the tiles fill the CUs (8192 x 1024 x 1024 fp32, 64 x 64 tiles: 144 us with two, 152 with three, 161 with four), and deep or wide
+//     stages where they do not (40 x 2048 x 2048 fp16: 12.3 -> 6.5 us with 8 waves sharing a 256-deep stage).
+//   * fp32 goes through the exact fp32 matrix instruction: 8192 x 1024 x 1024 at 131 TFLOP/s with 128 x 128 tiles.
+//   * 12013 x 61 x 512 fp32 (20 us; its stores alone take 6.3, its products 5.6, its loads 5.4): the three hardly overlap, since the workgroups of a CU
+//     start together; runs of column tiles, other tiles and deeper stages left it at 20 to 22 us.
+//   * odd strides (16 bit): a direct load wants 4-byte addresses; through registers 3001 x 777 x 1111 fp16 takes 18.3 us, 776 x 1112 14.8 directly.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -150,7 +164,7 @@ struct Stage {
     }
 };
 
-// The same straight into LDS: 16 bytes a lane, a wave fills 1 KB; the source of a lane is the piece that stands where the lane writes.
+// The same straight into LDS: 16 bytes a lane, a wave fills 1 KB without a register; the source of a lane is the piece that stands where the lane writes.
 // Sources have to be whole pieces (the address a multiple of 4 bytes); rows past the operand take the last one (their results are not stored).
 // The instruction is written out because the compiler's own form makes it wait for all such loads before any read of LDS; Core waits for them.
 __device__ __forceinline__ void direct16(const void* base, uint32_t voff, uint32_t lds) {
@@ -665,6 +679,7 @@ __global__ __launch_bounds__(ShX::THREADS) void grad_kernel(const ProductP x, co
 constexpr int64_t kMaxBlocks = (1 << 22) - 1;               // a grid has fewer than 2^32 work items, a workgroup up to 512
 constexpr int64_t kMaxStride = 1 << 22;                     // a tile's offsets fit 32 bits: 256 rows of 2^22 values
 constexpr int64_t kCus = 256;
+constexpr int kMaxGroups = 1 << 16;                         // every workgroup looks its group up among them, 64 at a time
 
 bool type_ok(int t) { return t == CT_F32 || t == CT_BF16 || t == CT_F16; }
 bool words(const void* p, int64_t ld, int64_t more, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size) | (uintptr_t)(more * size)) & 3) == 0; }
@@ -717,7 +732,7 @@ int launch(ProductP x, DwP w, hipStream_t st) {
     return (int)hipGetLastError();
 }
 
-// Shapes.  Named by their tile; measured (us) at the sizes given with the rules.
+// Shapes (tile, contraction steps of a stage, waves along m, n and the contraction, stages).  Two stages where tiles fill the CUs, for more workgroups on each.
 template <Way W> using T256 = Shape<256, 256, 64, 2, 4, 1, 2, W>;
 template <Way W> using T128 = Shape<128, 128, 64, 2, 4, 1, 2, W>;
 using T128run = Shape<128, 128, 64, 2, 4, 1, 2, DIRECT, 4>;
@@ -741,8 +756,18 @@ using R32k = Shape<32, 32, 256, 1, 1, 8, 2, REGS>;
 using Any = Shape<64, 64, 32, 2, 2, 1, 2, EDGE>;
 template <int BK> using AnyK = Shape<32, 32, BK, 1, 1, 8, 2, EDGE>;
 
-// Which tile.  16 x 64: a few rows a group, bound by the weights, every wave a quarter of the sum.  Large tiles where there are enough of them for all
-// CUs, since each value of an operand is then fetched less often; else small ones.
+// Which tile, by the rows a group has on average, the widths, and how many tiles that makes for 256 CUs.  Large tiles fetch each value less often, small
+// ones fill the card.  us, the chosen shape and the next best:
+//   16 bit   T256    32768 x 4096 x 2048, 16 groups   617 : 656 (128 x 128)        T128     8000 x 1024 x 1024, 8 groups    24.7 : 32.3 (128 x 64)
+//            T128run 30000 x 64 x 1024, 10 groups    25.2 : 30.1 (T128)            T128deep 3001 x 1112 x 776, 7 groups     19.6 : 20.9 (128 x 64)
+//            T64deep 500 x 2048 x 2048, 8 groups     15.5 : 20.8 (T64), 25.4 (T128) T64      8000 x 1024 x 1024, 8 groups    36.4 : 40.8 (T64deep)
+//            T32     1000 x 512 x 512, 4 groups       5.5 : 6.2 (T64)              T32k     100 x 3000 x 300, 4 groups       8.4 : 11.8 (T32)
+//            T32s    500 x 500 x 200, 30 groups       5.1 : 5.7 (T32)              T16      16 x 4096 x 512, 8 groups       11.3 : 13.9 (256-deep, two stages)
+//   fp32     F128    8192 x 1024 x 1024, 8 groups     131 : 144 (F64)              F64      3000 x 200 x 1500, 3 groups     28.7 : 33.2 (F32)
+//            F32     2048 x 512 x 512, 2 groups      13.3 : 14.3 (F32s)            F32s     1213 x 512 x 512, 2 groups      11.6 : 13.2 (F32)
+//            F16k    30 x 4000 x 100, 2 groups       18.7 : 28.3 (F32s)            F16      64 x 2048 x 256, 64 groups      24.1 : 26.3 (F32s)
+//   odd      T128    3001 x 777 x 1111 fp16, 7 groups 18.3 : 21.0 (128 x 64)       R64k     623 x 2755 x 838 fp16, 3 groups 26.7 : 36.9 (T64)
+//   any      AnyK    2 x 3181 x 16 fp32, 3 groups      37 : 138 (Any)
 template <typename TT, bool WT, Way WAY>
 int product_pick(const ProductP& p, hipStream_t st) {
     const int64_t mean = (p.rows + p.G - 1) / p.G, r = p.rows + p.G * 32;       // (a group's last tile is half full on average)
@@ -782,7 +807,8 @@ int product_pick(const ProductP& p, hipStream_t st) {
     if (k >= 512 && tiles(r, p.N, 32, 32) < 2 * kCus) return launch<TT, WT, AnyK<1024 / (int)sizeof(typename TT::S)>>(p, st);
     return launch<TT, WT, Any>(p, st);
 }
-// Few tiles with long sums: rows a part (0: the sums stay whole).  2 x 512 x 61 weights from 2 x 1024 rows are 16 tiles of 64 x 64.
+// Few tiles with long sums: rows a part (0: the sums stay whole).  61 x 512 weights in 2 groups from 1024 rows each are 16 tiles of 64 x 64: 8.7 us in
+// parts.  From 64 tiles on whole sums are faster: 512 x 512 in 2 groups from 1024 rows each (128 tiles), both gradients, 27.5 us whole, 35.3 in parts.
 int part_rows(int rows, int K, int N, int G) {
     const int64_t blocks = G * tiles(K, N, 64, 64), mean = rows / G;
     if (blocks >= 64 || mean < 512) return 0;
@@ -791,6 +817,7 @@ int part_rows(int rows, int K, int N, int G) {
 }
 int part_slots(int rows, int step, int G) { return rows / step + (rows < G ? rows : G); }
 
+// (128 x 128: 516 x 1022 in 9 groups, 2999 rows 12.1 us, 16.1 with 64 x 64; T64deep: 128 x 256 in 10 groups, 20000 rows 12.3 : 18.7 (T64))
 template <typename TT, Way WAY>
 int dw_pick(const DwP& p, hipStream_t st) {
     const int r = p.rows, k = p.K, n = p.N;
@@ -818,7 +845,7 @@ int dw_pick(const DwP& p, hipStream_t st) {
     }
     return launch<TT, Any>(p, st);
 }
-// Both gradients together where one shape suits them; x: dx as a product (its K is the width of dy, its N the width of x)
+// Both gradients together where one shape suits them (2999 x 515 x 1021 fp16 in 9 groups: 17.3 + 16.3 us apart, 27.1 together); x: dx as a product (its K is the width of dy, its N the width of x)
 template <typename TT, bool WT, Way WAY>
 int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     const int64_t mean = (x.rows + x.G - 1) / x.G, r = x.rows + x.G * 32;
@@ -887,7 +914,7 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0) return CT_EINVAL;
     if (rows == 0) return CT_OK;
     if (!offsets || !y || !x || !w || ldy < N || ldx < K || ldw < (w_transposed ? K : N) || w_group_stride < 0 || affine_stride < 0) return CT_EINVAL;
-    if (ldx > kMaxStride || ldw > kMaxStride) return CT_ESHAPE;
+    if (ldx > kMaxStride || ldw > kMaxStride || G > kMaxGroups) return CT_ESHAPE;
     const ProductP p{x, ldx, rows, K, w, w_group_stride, ldw, N, offsets, G, scale, shift, affine_stride, slope, fill_tail != 0, out_type == CT_F32, y, ldy, 0, 0, 0, 0};
     return product_any(type, p, w_transposed != 0, (hipStream_t)stream);
 }
@@ -904,7 +931,7 @@ int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0 || !offsets) return CT_EINVAL;
     if ((rows > 0 && !dy) || lddy < N || (dw && ((rows > 0 && !x) || ldx < K || lddw < N || dw_group_stride < (int64_t)(K - 1) * lddw + N))) return CT_EINVAL;
     if (dx && ((rows > 0 && !w) || ldw < (w_transposed ? K : N) || w_group_stride < 0 || lddx < K)) return CT_EINVAL;
-    if (lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
+    if (G > kMaxGroups || lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
     hipStream_t st = (hipStream_t)stream;
     const ProductP px{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0, 0};
     const int step = dw && rows > 0 ? part_rows(rows, K, N, G) : 0;

@@ -24,6 +24,7 @@ RATIO_SEG_ERROR = 0.15
 FFN_WEIGHTS_NAME = "weights_training_"
 k_ptrs = FFN_K_PTRS
 NUMBER_FEATURES = FFN_FEAT
+_uploading = threading.Lock()
 
 
 def flatten_ffn_weights(w: dict) -> np.ndarray:
@@ -40,14 +41,13 @@ class FFN:
         self._loaded = None            # the library's handle
         self._stale = False            # the training weights are ahead of it
         self._training = None
-        self._lock = threading.Lock()
         self._device = device
         self._weights = None
 
     @property
     def _handle(self):
         if self._stale:
-            with self._lock:                   # (matches run on several host threads: the first one brings the weights, the others wait)
+            with _uploading:                   # (matches run on several host threads: the first one brings the weights, the others wait)
                 if self._stale:
                     self._upload(self._training.weights())
                     self._stale = False

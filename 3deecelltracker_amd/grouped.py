@@ -15,7 +15,7 @@ from typing import Sequence, Union
 
 from . import _dev, _lib
 
-MAX_GROUPS = 1 << 20
+MAX_GROUPS = 1 << 16          # every workgroup looks its group up among them, 64 at a time
 _ready = None
 
 

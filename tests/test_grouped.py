@@ -70,6 +70,9 @@ CASES = [
     # the large tiles: more of them than compute units, partial in every direction
     ([4000, 0, 3500, 777], 72, 2050, 3), ([2100, 1, 2300], 136, 1161, 0), ([0, 90, 64, 131, 77, 1, 200, 63, 65, 2], 1300, 1290, 1),
     ([33, 0, 100, 5] * 4, 520, 517, 2), ([9] * 20 + [0] * 10 + [31], 700, 264, 2), ([40, 31], 2050, 70, 0),
+    # every rule by which a tile is chosen: runs of column tiles; deep and wide stages where tiles are few; both gradients in one launch
+    ([9000, 12000, 11000], 72, 650, 5), ([1500, 1500], 320, 900, 0), ([62, 63] * 4, 300, 1500, 2), ([250] * 4, 200, 512, 0), ([1024, 1024], 512, 512, 0),
+    ([4500, 4500], 40, 1000, 1), ([1] * 64, 200, 256, 0), ([300, 300], 515, 831, 0), ([3, 4] * 15, 333, 515, 0), ([250] * 14, 1300, 1290, 0), ([100] * 20, 300, 300, 3),
     # long sums for few columns, of even and odd width
     ([2, 0, 3], 3181, 16, 2), ([90, 1], 1024, 30, 0), ([100, 40], 1001, 333, 0), ([300, 41], 2755, 411, 1), ([33], 600, 1, 0),
     # long sums for few weights
@@ -302,6 +305,38 @@ def test_offsets_that_do_not_rise_stay_inside():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("groups", [64, 65, 1000, 20000])
+def test_many_groups(groups):
+    t = _torch()
+    rng = np.random.default_rng(groups)
+    counts = np.bincount(rng.integers(0, groups, 300), minlength=groups).tolist()
+    x, w = _rand((300, 48), "bfloat16", 1), _rand((groups, 48, 32), "bfloat16", 2, 0.2)
+    y = grouped.product(x, w, _offsets(counts))
+    group = np.repeat(np.arange(groups), counts)
+    xs, ws = x.double().cpu(), w.double().cpu()[group]
+    _check(y, (xs[:, None] @ ws)[:, 0], (52 * UNIT) * (xs.abs()[:, None] @ ws.abs())[:, 0], y.dtype)
+    dw = grouped.product_grad(y, x, w, _offsets(counts), need_x=False)[1]
+    assert bool((dw[t.tensor(counts, device="cuda") == 0] == 0).all())
+    one = int(np.argmax(counts)); a = _offsets(counts)[one]; b = a + counts[one]
+    ys = y[a:b].double().cpu()
+    _check(dw[one], xs[a:b].T @ ys, ((b - a + 4) * UNIT) * (xs[a:b].abs().T @ ys.abs()), dw.dtype)
+
+
+@pytest.mark.gpu
+def test_gradients_of_a_shared_block():
+    t = _torch()
+    counts, w = [50, 0, 70], _rand((1, 61, 40), "float32", 1)
+    x, dy = _rand((120, 61), "float32", 2), _rand((120, 40), "float32", 3)
+    dx, dw = grouped.product_grad(dy, x, w.expand(3, 61, 40), _offsets(counts))
+    want, bound = _ref(dy, w.expand(3, 61, 40).transpose(1, 2), counts)
+    _check(dx, want, bound, dx.dtype)
+    whole = grouped.product_grad(dy, x, w, [0, 120])[1]
+    xs, ds = x.double().cpu(), dy.double().cpu()
+    _check(dw.sum(0, keepdim=True), (xs.T @ ds)[None], (2 * 124 * UNIT) * (xs.abs().T @ ds.abs())[None], t.float32)
+    _check(whole, (xs.T @ ds)[None], (124 * UNIT) * (xs.abs().T @ ds.abs())[None], t.float32)
+
+
+@pytest.mark.gpu
 def test_empty_batch():
     t = _torch()
     x, w = t.empty(0, 61, device="cuda"), _rand((2, 61, 16), "float32", 1)
@@ -346,7 +381,7 @@ def test_the_abi_refuses_without_a_gpu():
     for kw in (dict(type=3), dict(type=-1), dict(out=1), dict(rows=-1), dict(K=0), dict(N=0), dict(G=0), dict(x=None), dict(w=None), dict(off=None), dict(y=None),
                dict(ldx=7), dict(ldw=5), dict(ldy=5), dict(wg=-1), dict(ag=-1), dict(wt=1, ldw=7)):
         assert call(**kw) == _lib.CT_EINVAL, kw
-    assert call(rows=0) == 0
+    assert call(rows=0) == 0 and call(G=2 ** 16 + 1) == _lib.CT_ESHAPE
     assert call(rows=2 ** 31 - 1, N=2 ** 20, ldw=2 ** 20, ldy=2 ** 20) == _lib.CT_ESHAPE
     ok2 = dict(type=0, out=0, dy=64, lddy=6, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, dx=64, lddx=8, dw=64, dwg=48, lddw=6, ws=None,
                wsb=0, st=None)
