@@ -77,6 +77,10 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
     return t.tensor(host, dtype=t.int32).to(device)
 
 
+def _as_is(t, a, groups, n, device):
+    return a is None or (isinstance(a, t.Tensor) and a.shape == (groups, n) and a.dtype is t.float32 and a.device == device and a.is_contiguous())
+
+
 def _affine(name, a, groups, n, device):
     """[n] or [groups, n] -> (tensor with contiguous rows, stride of its groups)"""
     t = _env()[0]
@@ -143,7 +147,11 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
     off = offsets_device(offsets, g, rows, device)
     sc = sh = None
     stride = 0
-    if scale is not None or shift is not None:
+    if scale is None and shift is None:
+        pass
+    elif _as_is(t, scale, g, n, device) and _as_is(t, shift, g, n, device):
+        sc, sh, stride = scale, shift, n
+    else:
         (sc, s1), (sh, s2) = ((None, None) if a is None else _affine(name, a, g, n, device) for name, a in (("scale", scale), ("shift", shift)))
         if s1 is not None and s2 is not None and s1 != s2:            # one for all groups, the other for each
             sc, sh, s1 = sc.expand(g, n).contiguous(), sh.expand(g, n).contiguous(), n
