@@ -746,7 +746,7 @@ using T32s = Shape<32, 32, 128, 1, 1, 4, 3, DIRECT>;
 using T16 = Shape<16, 64, 128, 1, 1, 4, 4, DIRECT>;
 using T16r = Shape<16, 64, 128, 1, 1, 4, 2, REGS>;
 using F128 = Shape<128, 128, 32, 2, 4, 1, 2, DIRECT>;
-using F64 = Shape<64, 64, 32, 2, 2, 1, 2, DIRECT>;
+using F64 = Shape<64, 64, 32, 2, 4, 1, 2, DIRECT>;
 using F32 = Shape<32, 64, 64, 1, 1, 4, 2, DIRECT>;
 using F32s = Shape<32, 32, 64, 1, 1, 4, 2, DIRECT>;
 using F16 = Shape<16, 64, 128, 1, 1, 4, 2, DIRECT>;
@@ -763,10 +763,10 @@ template <int BK> using AnyK = Shape<32, 32, BK, 1, 1, 8, 2, EDGE>;
 //            T64deep 500 x 2048 x 2048, 8 groups     15.5 : 20.8 (T64), 25.4 (T128) T64      8000 x 1024 x 1024, 8 groups    36.4 : 40.8 (T64deep)
 //            T32     1000 x 512 x 512, 4 groups       5.5 : 6.2 (T64)              T32k     100 x 3000 x 300, 4 groups       8.4 : 11.8 (T32)
 //            T32s    500 x 500 x 200, 30 groups       5.1 : 5.7 (T32)              T16      16 x 4096 x 512, 8 groups       11.3 : 13.9 (256-deep, two stages)
-//   fp32     F128    8192 x 1024 x 1024, 8 groups     131 : 144 (F64)              F64      3000 x 200 x 1500, 3 groups     28.7 : 33.2 (F32)
+//   fp32     F128    8192 x 1024 x 1024, 8 groups     131 : 136 (F64)              F64      3000 x 200 x 1500, 3 groups     28.0 : 29.6 (4 waves), 33.2 (F32)
 //            F32     2048 x 512 x 512, 2 groups      13.3 : 14.3 (F32s)            F32s     1213 x 512 x 512, 2 groups      11.6 : 13.2 (F32)
 //            F16k    30 x 4000 x 100, 2 groups       18.7 : 28.3 (F32s)            F16      64 x 2048 x 256, 64 groups      24.1 : 26.3 (F32s)
-//   odd      T128    3001 x 777 x 1111 fp16, 7 groups 18.3 : 21.0 (128 x 64)       R64k     623 x 2755 x 838 fp16, 3 groups 26.7 : 36.9 (T64)
+//   odd      T128    3001 x 777 x 1111 fp16, 7 groups 18.3 : 21.0 (128 x 64)       R64k     500 x 2047 x 2047 fp16, 8 groups 22.7 : 28.7 (T64)
 //   any      AnyK    2 x 3181 x 16 fp32, 3 groups      37 : 138 (Any)
 template <typename TT, bool WT, Way WAY>
 int product_pick(const ProductP& p, hipStream_t st) {
@@ -790,7 +790,7 @@ int product_pick(const ProductP& p, hipStream_t st) {
         if (k >= 512 && n >= 32 && tiles(r, p.N, 32, 32) < 2 * kCus) return launch<TT, WT, R32k>(p, st);
         if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, T16r>(p, st);
         if (mean >= 96 && k >= 64 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 160) return launch<TT, WT, T128<REGS>>(p, st);
-        if (k >= 512 && n >= 64 && tiles(r, p.N, 64, 64) < kCus) return launch<TT, WT, R64k>(p, st);
+        if (k >= 512 && n >= 64 && tiles(r, p.N, 64, 64) <= 2 * kCus) return launch<TT, WT, R64k>(p, st);
         if (k >= 64 && n >= 64) return launch<TT, WT, T64<REGS>>(p, st);
         if (k >= 32 && n >= 64) return launch<TT, WT, T64flat<REGS>>(p, st);
     }
