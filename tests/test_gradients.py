@@ -81,6 +81,16 @@ def test_large_tensors_repeat_bit_for_bit():
 
 
 @pytest.mark.gpu
+def test_a_tensor_past_32_bits():
+    t = _torch()
+    g = t.zeros(2 ** 31 + 4101, dtype=t.bfloat16, device="cuda")
+    g[-3:] = t.tensor([3.0, -4.0, 12.0], device="cuda"); g[1] = 84.0
+    out, norm = gradients.clip_by_global_norm([g], 8.5)
+    assert float(norm) == 85.0 and out[0][-3:].tolist() == [0.30078125, -0.400390625, 1.203125] and float(out[0][1]) == 8.375   # a tenth, rounded to bf16
+    assert int(t.count_nonzero(out[0])) == 4
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("offset", [0, 1, 2, 3, 5, 8])
 def test_slices_of_one_buffer(offset):
     """Gradients end to end in a bucket: any alignment of a value; what lies between them stays as it was"""

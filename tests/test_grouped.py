@@ -291,6 +291,33 @@ def test_offsets_on_the_device_and_streams_and_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_sums_in_parts_in_a_graph_with_other_groups(dtype):
+    """Long sums for few weights: the parts of each group are counted on the device, whatever the offsets hold when the graph is replayed"""
+    t = _torch()
+    x, dy, w = _rand((4000, 61), dtype, 1), _rand((4000, 70), dtype, 2, 0.1), _rand((3, 61, 70), dtype, 3, 0.1)
+    off = t.tensor([0, 2000, 2000, 4000], dtype=t.int32, device="cuda")
+    grouped.product_grad(dy, x, w, off)
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        dx, dw = grouped.product_grad(dy, x, w, off, out_dtype=t.float32)
+    xs, ds = x.double().cpu(), dy.double().cpu()
+    for o in ([0, 2000, 2000, 4000], [0, 0, 0, 4000], [0, 1, 2, 3], [0, 4000, 4000, 4000], [0, 1333, 2666, 3999], [0, 0, 0, 0]):
+        off.copy_(t.tensor(o, dtype=t.int32))
+        graph.replay()
+        t.cuda.synchronize()
+        want = t.stack([xs[a:b].T @ ds[a:b] for a, b in zip(o, o[1:])])
+        bound = t.stack([(b - a + 4) * UNIT * (xs[a:b].abs().T @ ds[a:b].abs()) for a, b in zip(o, o[1:])])
+        _check(dw, want, bound, t.float32)
+        ex, ew = grouped.product_grad(dy, x, w, off, out_dtype=t.float32)
+        assert t.equal(dw, ew) and t.equal(dx, ex)
+    for o in ([0, 3900, 10, 4000], [4000, 0, 4000, 0]):                  # not rising: any values, nothing outside
+        off.copy_(t.tensor(o, dtype=t.int32))
+        graph.replay()
+        t.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_offsets_that_do_not_rise_stay_inside():
     """Numbers on the device are not looked at by the host: whatever they hold, nothing outside the result is written"""
     t = _torch()
