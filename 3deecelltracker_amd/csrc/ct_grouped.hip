@@ -845,7 +845,8 @@ int dw_pick(const DwP& p, hipStream_t st) {
     }
     return launch<TT, Any>(p, st);
 }
-// Both gradients together where one shape suits them (2999 x 515 x 1021 fp16 in 9 groups: 17.3 + 16.3 us apart, 27.1 together); x: dx as a product (its K is the width of dy, its N the width of x)
+// Both gradients together where one shape suits them (2999 x 515 x 1021 fp16 in 9 groups: 17.3 + 16.3 us apart, 27.1 together; 200 x 300 x 500 fp16 in 30
+// groups 12.4 apart, 8.3 together; the worst found is 300 x 128 x 1000 fp32 in 40 groups, 22.5 and 24.6, with 2.2 us less on the host); x: dx as a product (its K is the width of dy, its N the width of x)
 template <typename TT, bool WT, Way WAY>
 int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     const int64_t mean = (x.rows + x.G - 1) / x.G, r = x.rows + x.G * 32;
@@ -855,11 +856,11 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
         if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return launch<TT, WT, T256<WAY>, T256<WAY>>(x, w, st);
     if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
         if (mean >= 96 && least >= 128 && sum(128) >= kCus) return launch<TT, WT, T128<WAY>, T128<WAY>>(x, w, st);
-        if (mean > 16 && x.rows >= 64 && least >= 64) return launch<TT, WT, T64<WAY>, T64<WAY>>(x, w, st);
+        if (x.rows >= 64 && least >= 64) return launch<TT, WT, T64<WAY>, T64<WAY>>(x, w, st);
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
         if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
-        if (mean > 16 && x.rows >= 64 && least >= 64) {
+        if (x.rows >= 64 && least >= 64) {
             // 32 x 64 tiles (48 KB: 3 on a CU) where they all run at once and fill it: 2048 x 512 x 512 in 2 groups 23.3 us, 27.4 with 32 x 32;
             // 500 x 200 x 1000 in 4 groups 16.9, 12.8 with 32 x 32
             const int64_t n64 = tiles(r, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64);
