@@ -283,7 +283,8 @@ struct Core {
     static constexpr int STAGE_BYTES = TA::BYTES + TB::BYTES, SUM_BYTES = WK > 1 ? BM * BN * WK * 4 : 0;
     static constexpr int LDS_BYTES = NB * STAGE_BYTES > SUM_BYTES ? NB * STAGE_BYTES : SUM_BYTES;
     static_assert(WAY == DIRECT || NB == 2, "registers hold one stage");
-    // fp32 sums of one wave run over at most kChain steps and are then added to the total: a long chain loses a bit for every fourfold length
+    // fp32 sums of one wave run over at most kChain steps and are then added to the total: a long chain loses a bit for every fourfold length (7542 x 2809 x
+    // 708: 3.9e-7 of the norm, 9.3e-7 as one chain).  Not where waves share a sum: theirs are a quarter as long (4096 steps: 5.7e-7; 4.1e-7 with it, 5 to 15 % slower)
     static constexpr int kChain = 512;
     static constexpr bool FOLD = !H && WK == 1;
     typedef typename std::conditional<H, s16x8, f32x4>::type Frag;
