@@ -170,7 +170,7 @@ struct Stage {
 // A load does not wait for a base that a v_readfirstlane has just written: that takes five wait states (s_mov and s_nop 3), which the compiler counts for
 // its own loads only; scripts/check_sgpr_waits.py holds the built code to it.
 __device__ __forceinline__ void direct16(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(voff), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(voff), "s"(base) : "m0", "memory");
 }
 template <typename S, bool CC, int E, int BK, int NT>
 struct Direct {

@@ -37,3 +37,14 @@ def test_no_load_takes_an_address_too_early(waits):
     if not (CSRC / "ct_grouped.o").exists():
         importlib.import_module("__graft_entry__").build()
     assert waits.check() == {}
+
+
+def test_inline_assembly_names_the_registers_it_writes():
+    """m0 and the condition registers are written by name, not through an output: the compiler knows only what the clobber list says"""
+    import re
+    for source in sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.h")):
+        for m in re.finditer(r"\basm\s*(?:volatile)?\s*\((.*?)\)\s*;", re.sub(r"//[^\n]*", "", source.read_text()), flags=re.S):
+            text = m.group(1)
+            code, _, lists = text.partition(":")
+            for register in re.findall(r"\b(m0|vcc|exec|scc)\b\s*,", code):
+                assert f'"{register}"' in lists, f"{source.name}: {text}"
