@@ -24,7 +24,6 @@ RATIO_SEG_ERROR = 0.15
 FFN_WEIGHTS_NAME = "weights_training_"
 k_ptrs = FFN_K_PTRS
 NUMBER_FEATURES = FFN_FEAT
-_uploading = threading.Lock()
 
 
 def flatten_ffn_weights(w: dict) -> np.ndarray:
@@ -43,19 +42,21 @@ class FFN:
         self._training = None
         self._device = device
         self._weights = None
+        self._lock = threading.RLock()         # held wherever the weights change: training steps, uploads, new weights
 
     @property
     def _handle(self):
         if self._stale:
-            with _uploading:                   # (matches run on several host threads: the first one brings the weights, the others wait)
+            with self._lock:                   # (matches run on several host threads: the first one brings the weights, the others wait)
                 if self._stale:
                     self._upload(self._training.weights())
                     self._stale = False
         return self._loaded
 
     def set_weights_dict(self, w: dict):
-        self._training, self._stale = None, False
-        return self._upload(w)
+        with self._lock:
+            self._training, self._stale = None, False
+            return self._upload(w)
 
     def _upload(self, w: dict):
         t = _lib.require_gpu()
@@ -93,8 +94,9 @@ class FFN:
         """Start training from the present weights: Adam, binary cross-entropy, all gradients clipped together by `global_clipnorm` (Keras' names and
         defaults; the loop around it, reference ffn.py:56-222, is the caller's)."""
         from .ffn_training import FFNTraining
-        self._require()
-        self._training = FFNTraining(self._weights, f"cuda:{self._device}", learning_rate, beta_1, beta_2, epsilon, global_clipnorm)
+        with self._lock:
+            self._require()
+            self._training = FFNTraining(self._weights, f"cuda:{self._device}", learning_rate, beta_1, beta_2, epsilon, global_clipnorm)
 
     def train_on_batch(self, x, y) -> float:
         """One update from x -- (P,122), or the two halves [ (P,61), (P,61) ] -- and labels y (P,) or (P,1) in [0, 1]; numpy or torch -> the loss
@@ -108,14 +110,18 @@ class FFN:
         y = _dev.to_dev(y, t.float32, f"cuda:{self._device}").reshape(-1)
         if x.ndim != 2 or x.shape[1] != 2 * FFN_FEAT or x.shape[0] < 2 or y.shape[0] != x.shape[0]:
             raise ValueError(f"expected at least two rows (P, {2 * FFN_FEAT}) and as many labels, got {tuple(x.shape)} and {tuple(y.shape)}")
-        with t.cuda.device(x.device):
-            loss = self._training.step(x, y)
-        self._stale = True
-        return float(loss)
+        with self._lock:
+            if self._training is None:
+                raise ValueError("FFN is not being trained: its weights were replaced meanwhile")
+            with t.cuda.device(x.device):
+                loss = self._training.step(x, y)
+            self._stale = True
+            return float(loss)                                            # (waits for the update: weights() may read it on another stream)
 
     def save_weights(self, path):
-        self._handle                                                      # (training weights come back first)
-        w = self._weights
+        with self._lock:
+            self._handle                                                  # (training weights come back first)
+            w = self._weights
         if w is None:
             raise ValueError("model has no weights")
         out = {"w1": w["w1"], "w2": w["w2"], "w3": w["w3"], "b3": w["b3"]}

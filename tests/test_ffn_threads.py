@@ -1,0 +1,104 @@
+"""CPU-only: the matching network's weights when training steps, uploads and matches meet on several host threads (the library and the training
+step are stand-ins that say when they run)."""
+import contextlib
+import importlib
+import threading
+
+import numpy as np
+import pytest
+
+ffn_mod = importlib.import_module("3deecelltracker_amd.ffn")
+_dev = importlib.import_module("3deecelltracker_amd._dev")
+_lib = importlib.import_module("3deecelltracker_amd._lib")
+WAIT = 0.3          # how long a thread is given to do what it must not do
+
+
+class Training:
+    """Counts steps; `during_step` and `during_weights` run in the middle of either"""
+
+    def __init__(self):
+        self.version, self.stepping, self.torn = 0, False, 0
+        self.during_step = self.during_weights = lambda: None
+
+    def step(self, x, y):
+        self.stepping = True
+        self.version += 1
+        self.during_step()
+        self.stepping = False
+        return 0.5
+
+    def weights(self):
+        self.torn += self.stepping
+        version = self.version
+        self.during_weights()
+        return {"version": version}
+
+
+@pytest.fixture
+def model(monkeypatch):
+    import torch
+    monkeypatch.setattr(_lib, "require_gpu", lambda: torch)
+    monkeypatch.setattr(_dev, "to_dev", lambda a, dtype, device=None: torch.as_tensor(a, dtype=dtype))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    m = ffn_mod.FFN(device=0)
+
+    def upload(w):
+        m._loaded, m._weights = ("handle", w.get("version")), w
+        return m
+    monkeypatch.setattr(m, "_upload", upload)
+    m._training = Training()
+    return m
+
+
+def _step(m):
+    m.train_on_batch(np.zeros((2, 122), np.float32), np.zeros(2, np.float32))
+
+
+def _beside(call):
+    """call() on another thread, given some time; -> the thread"""
+    t = threading.Thread(target=call)
+    t.start()
+    t.join(WAIT)
+    return t
+
+
+def test_a_step_during_an_upload_is_not_lost(model):
+    _step(model)
+    threads = []
+
+    def once():
+        model._training.during_weights = lambda: None
+        threads.append(_beside(lambda: _step(model)))
+    model._training.during_weights = once
+    first = model._handle                                  # brings step 1; step 2 arrives while it is being copied
+    threads[0].join()
+    assert first[1] in (1, 2) and model._training.version == 2
+    assert model._handle == ("handle", 2)
+
+
+def test_weights_are_not_copied_in_the_middle_of_a_step(model):
+    _step(model)
+    threads, seen = [], []
+
+    def once():
+        model._training.during_step = lambda: None
+        threads.append(_beside(lambda: seen.append(model._handle)))
+    model._training.during_step = once
+    _step(model)
+    threads[0].join()
+    assert model._training.torn == 0 and model._handle == ("handle", 2) and seen == [("handle", 2)]
+
+
+def test_the_update_is_waited_for_before_another_thread_may_copy_it(model):
+    """The loss comes from the training thread's stream; until it is there, the update may still run"""
+    threads = []
+
+    class Loss:
+        def __float__(self):
+            threads.append(_beside(lambda: model._handle))
+            assert model._loaded is None, "copied before the update was waited for"
+            return 0.5
+    model._training.step = lambda x, y: Loss()
+    _step(model)
+    threads[0].join()
+    assert model._loaded == ("handle", 0)
