@@ -32,12 +32,24 @@ def flatten_ffn_weights(w: dict) -> np.ndarray:
     return np.ascontiguousarray(np.concatenate([np.asarray(p, dtype=np.float32).ravel() for p in parts]))
 
 
+class _Loaded:
+    """A handle of the library as ctypes passes it.  A call that was given it keeps it: it is destroyed when the last one has returned, not when
+    other weights take its place (its memory is freed behind everything that the device has been asked to do by then)."""
+
+    def __init__(self, handle):
+        self._as_parameter_ = handle
+        self._destroy = _lib.lib().ct_ffn_destroy
+
+    def __del__(self):
+        self._destroy(self._as_parameter_)
+
+
 class FFN:
     """Dense(61->512, no bias)+BN+LeakyReLU shared by both halves, concat, Dense(1024->512, no
     bias)+BN+LeakyReLU, Dense(512->1)+sigmoid -- evaluated by the HIP library."""
 
     def __init__(self, device: int | None = None):
-        self._loaded = None            # the library's handle
+        self._loaded = None            # the library's handle (_Loaded)
         self._stale = False            # the training weights are ahead of it
         self._training = None
         self._device = device
@@ -66,10 +78,9 @@ class FFN:
         L = _lib.lib()
         if flat.size != L.ct_ffn_num_weights():
             raise ValueError(f"FFN weight count {flat.size} != {L.ct_ffn_num_weights()}")
-        self._free()
         h = C.c_void_p()
         _lib.check(L.ct_ffn_create(flat.ctypes.data, flat.size, self._device, C.byref(h)), "ct_ffn_create")
-        self._loaded = h
+        self._loaded = _Loaded(h)
         self._weights = w
         return self
 
@@ -167,17 +178,6 @@ class FFN:
         return out
 
     __call__ = predict
-
-    def _free(self):
-        if self._loaded is not None:
-            _lib.lib().ct_ffn_destroy(self._loaded)
-            self._loaded = None
-
-    def __del__(self):
-        try:
-            self._free()
-        except Exception:
-            pass
 
 
 def initial_matching_device(ffn_model: FFN, ref_d, tgt_d, k: int = FFN_K_PTRS):

@@ -1,6 +1,7 @@
 """CPU-only: the matching network's weights when training steps, uploads and matches meet on several host threads (the library and the training
 step are stand-ins that say when they run)."""
 import contextlib
+import ctypes
 import importlib
 import threading
 
@@ -102,3 +103,61 @@ def test_the_update_is_waited_for_before_another_thread_may_copy_it(model):
     _step(model)
     threads[0].join()
     assert model._loaded == ("handle", 0)
+
+
+class Library:
+    """Handles as numbers; a call reports which of them live while it runs"""
+
+    def __init__(self):
+        self.alive, self.made, self.inside = set(), 0, None
+        keep = self
+
+        class Entry:
+            def __call__(self, handle, *rest):
+                ctypes.c_void_p.from_param(handle)         # what ctypes asks of an argument
+                number = getattr(handle, "_as_parameter_", handle).value
+                if keep.inside:
+                    keep.inside()
+                assert number in keep.alive, f"handle {number} was destroyed during a call"
+                return 0
+        self.ct_ffn_pairgrid = Entry()
+
+    def ct_ffn_num_weights(self):
+        return 3
+
+    def ct_ffn_workspace_bytes(self, n, m):
+        return 16
+
+    def ct_ffn_create(self, w, n, device, out):
+        self.made += 1
+        self.alive.add(self.made)
+        out._obj.value = self.made
+        return 0
+
+    def ct_ffn_destroy(self, handle):
+        self.alive.discard(getattr(handle, "value", handle))
+
+
+@pytest.fixture
+def library(monkeypatch):
+    import torch
+    lib = Library()
+    monkeypatch.setattr(_lib, "require_gpu", lambda: torch)
+    monkeypatch.setattr(_lib, "lib", lambda: lib)
+    monkeypatch.setattr(_dev, "stream", lambda d: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(ffn_mod, "flatten_ffn_weights", lambda w: np.zeros(w["size"], np.float32))
+    return lib
+
+
+def test_a_match_in_flight_keeps_its_weights(library):
+    import torch
+    m = ffn_mod.FFN(device=0)
+    m.set_weights_dict({"size": 3})
+    library.inside = lambda: m.set_weights_dict({"size": 3})
+    m.pairgrid_device(torch.zeros(4, 61), torch.zeros(4, 61))
+    library.inside = None
+    assert library.alive == {2}                            # and the first handle is gone once the call has returned
+    m.pairgrid_device(torch.zeros(4, 61), torch.zeros(4, 61))
+    del m
+    assert library.alive == set()
