@@ -67,8 +67,9 @@ class FFN:
 
     def set_weights_dict(self, w: dict):
         with self._lock:
+            self._upload(w)                    # (weights that do not fit are refused: everything is as it was then, training too)
             self._training, self._stale = None, False
-            return self._upload(w)
+            return self
 
     def _upload(self, w: dict):
         t = _lib.require_gpu()

@@ -161,3 +161,15 @@ def test_a_match_in_flight_keeps_its_weights(library):
     m.pairgrid_device(torch.zeros(4, 61), torch.zeros(4, 61))
     del m
     assert library.alive == set()
+
+
+def test_weights_that_are_refused_change_nothing(library):
+    m = ffn_mod.FFN(device=0)
+    m.set_weights_dict({"size": 3})
+    m._training = training = Training()
+    training.weights = lambda: {"size": 3, "trained": True}
+    m._stale = True                                        # a step ahead of the library's handle
+    with pytest.raises(ValueError):
+        m.set_weights_dict({"size": 4})
+    assert m._training is training
+    assert m._handle._as_parameter_.value == 2 and m._weights["trained"]
