@@ -61,7 +61,8 @@ class FFN:
         if self._stale:
             with self._lock:                   # (matches run on several host threads: the first one brings the weights, the others wait)
                 if self._stale:
-                    self._upload(self._training.weights())
+                    with _lib.require_gpu().cuda.device(self._device):       # (creating a handle makes its device current: loading weights does, reading them does not)
+                        self._upload(self._training.weights())
                     self._stale = False
         return self._loaded
 

@@ -173,3 +173,28 @@ def test_weights_that_are_refused_change_nothing(library):
         m.set_weights_dict({"size": 4})
     assert m._training is training
     assert m._handle._as_parameter_.value == 2 and m._weights["trained"]
+
+
+def test_reading_the_handle_leaves_the_current_device_alone(library, monkeypatch):
+    import torch
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d
+        yield
+        current[0] = before
+    create = library.ct_ffn_create
+
+    def create_there(w, n, where, out):
+        current[0] = where                                 # what the library does
+        return create(w, n, where, out)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(library, "ct_ffn_create", create_there)
+    m = ffn_mod.FFN(device=3)
+    m.set_weights_dict({"size": 3})
+    assert current == [3]                                  # (as ever: points that are uploaded next go where the weights are)
+    m._training = Training()
+    m._training.weights = lambda: {"size": 3}
+    current[0], m._stale = 1, True
+    assert m._handle is not None and current == [1] and library.made == 2
