@@ -56,6 +56,13 @@ class FFN:
         self._weights = None
         self._lock = threading.RLock()         # held wherever the weights change: training steps, uploads, new weights
 
+    def __getstate__(self):                    # (a model without weights can be copied and sent to a worker; a handle refuses)
+        return {k: v for k, v in self.__dict__.items() if k != "_lock"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._lock = threading.RLock()
+
     @property
     def _handle(self):
         if self._stale:

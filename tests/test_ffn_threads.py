@@ -198,3 +198,11 @@ def test_reading_the_handle_leaves_the_current_device_alone(library, monkeypatch
     m._training.weights = lambda: {"size": 3}
     current[0], m._stale = 1, True
     assert m._handle is not None and current == [1] and library.made == 2
+
+
+def test_a_model_without_weights_can_be_copied(library):
+    import copy
+    import pickle
+    for m in (copy.deepcopy(ffn_mod.FFN(device=0)), pickle.loads(pickle.dumps(ffn_mod.FFN(device=0)))):
+        m.set_weights_dict({"size": 3})
+        assert m._handle is not None and m._device == 0
