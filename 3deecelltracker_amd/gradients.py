@@ -11,7 +11,9 @@ import ctypes as C
 import math
 
 from . import _dev, _lib
-from .grouped import _env, _on_device
+from .grouped import _capturing, _env, _on_device
+
+_captured: list = []          # the tables that a graph reads: it may be replayed after its set is gone (40 bytes a tensor each)
 
 
 def _dense(a):
@@ -72,7 +74,8 @@ class GradientSet:
     grads: float32, bfloat16 and float16 tensors of one device, mixed as they come, of any shape (also without values); each must fill its
     memory (contiguous, or with its indices in another order).  out: where clip() writes, tensors of the same type and layout; left out,
     the gradients are clipped in place.  The set holds the tensors; it has to be made anew when one of them is replaced.  Making it waits for
-    the current stream (the list is then ready for every stream), so it cannot be made while a graph is captured; its calls can be."""
+    the current stream (the list is then ready for every stream), so it cannot be made while a graph is captured; its calls can be.  A set may
+    be dropped while its calls are on their way on any stream; a graph that captured one needs the gradients and `out` to stay, as graphs do."""
 
     def __init__(self, grads, out=None):
         self._init(grads, out)
@@ -93,14 +96,30 @@ class GradientSet:
         ins = (C.c_void_p * m)(*[g.data_ptr() for g in self.grads])
         outs = (C.c_void_p * m)(*[o.data_ptr() for o in self.out])
         self._chunks = L.ct_gradset_chunks(n, sizes)
+        self._keeps, self._streams = once, {t._C._cuda_getCurrentRawStream(self._device.index)}
         with t.cuda.device(self._device):
             self._table = _dev.workspace(L.ct_gradset_table_bytes(n), self._device)
             _lib.check(L.ct_gradset_write(n, ins, outs, sizes, types, self._table.data_ptr(), self._table.numel(), _dev.stream(self._device)),
                        "ct_gradset_write")
         self._ws, self._at = L.ct_gradset_workspace_bytes(), self._table.data_ptr()
 
+    def _used_on(self, t, stream):
+        """The memory that a call on a stream other than the list's own reads and writes is not handed out again before that stream is through"""
+        with t.cuda.device(self._device):
+            current = t.cuda.current_stream()
+            for a in {id(a): a for a in (self._table, *self.grads, *self.out)}.values():
+                a.record_stream(current)
+        self._streams.add(stream)
+
     def _call(self, call, *args):
         t = _env()[0]
+        stream = t._C._cuda_getCurrentRawStream(self._device.index)
+        if _capturing(t, self._device):
+            if not self._keeps:
+                _captured.append(self._table)
+                self._keeps = True
+        elif stream not in self._streams:
+            self._used_on(t, stream)
         # the scalar and the partial sums, new for each call: two streams, or two graphs, share none
         scalar, ws = t.empty((), dtype=t.float32, device=self._device), t.empty(self._ws, dtype=t.uint8, device=self._device)
         rc = _on_device(t, self._device, call, self._at, self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws)

@@ -124,6 +124,14 @@ def _on_device(t, device, call, *args):
         return call(*args, t._C._cuda_getCurrentRawStream(device.index))
 
 
+def _capturing(t, device):
+    """Whether the current stream of `device` is being captured into a graph"""
+    if t._C._cuda_getDevice() == device.index:
+        return t._C._cuda_isCurrentStreamCapturing()
+    with t.cuda.device(device):
+        return t._C._cuda_isCurrentStreamCapturing()
+
+
 def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, slope: float = 1.0, out=None, out_dtype=None):
     """y[r] = act(scale[g] * (x[r] . w[g]) + shift[g]) for the rows offsets[g] <= r < offsets[g + 1]; act(v) = v or slope * v where v < 0.
 
