@@ -88,7 +88,7 @@ class GradientSet:
         self._n = len(self.grads)
         if self._device is None:                              # an empty list: its norm is zero, on the current device
             self._device = t.device("cuda", t.cuda.current_device())
-        if not once and t.cuda.is_current_stream_capturing():
+        if not once and _capturing(t, self._device):
             raise ValueError("GradientSet: make the set before the capture begins")
         n, m = self._n, max(self._n, 1)
         sizes = (C.c_int64 * m)(*[g.numel() for g in self.grads])

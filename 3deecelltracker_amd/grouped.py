@@ -57,6 +57,14 @@ def _row_stride(name, rows, cols, row_stride, col_stride):
     return row_stride
 
 
+def _capturing(t, device):
+    """Whether the current stream of `device` is being captured into a graph"""
+    if t._C._cuda_getDevice() == device.index:
+        return t._C._cuda_isCurrentStreamCapturing()
+    with t.cuda.device(device):
+        return t._C._cuda_isCurrentStreamCapturing()
+
+
 def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, rows: int, device):
     """int32 [groups + 1] on `device`.  Numbers on the host (a sequence, an array, a CPU tensor) are checked and uploaded; a tensor that is on
     the device already (a router's counts, summed there) is taken as it is, since looking at it would wait for the stream."""
@@ -72,7 +80,7 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
         raise ValueError(f"offsets: expected {groups + 1} numbers for {groups} groups, got {len(host)}")
     if host[0] != 0 or any(a > b for a, b in zip(host, host[1:])) or host[-1] > rows:
         raise ValueError(f"offsets: must rise from 0 to at most {rows} rows")
-    if t.cuda.is_current_stream_capturing():
+    if _capturing(t, device):
         raise ValueError("offsets: numbers on the host cannot be uploaded while a graph is captured; pass an int32 tensor on the device")
     return t.tensor(host, dtype=t.int32).to(device)
 
@@ -122,14 +130,6 @@ def _on_device(t, device, call, *args):
         return call(*args, t._C._cuda_getCurrentRawStream(device.index))
     with t.cuda.device(device):
         return call(*args, t._C._cuda_getCurrentRawStream(device.index))
-
-
-def _capturing(t, device):
-    """Whether the current stream of `device` is being captured into a graph"""
-    if t._C._cuda_getDevice() == device.index:
-        return t._C._cuda_isCurrentStreamCapturing()
-    with t.cuda.device(device):
-        return t._C._cuda_isCurrentStreamCapturing()
 
 
 def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, slope: float = 1.0, out=None, out_dtype=None):

@@ -1,0 +1,69 @@
+"""CPU-only: what cannot be done while a graph is captured is refused by the stream of the tensors' device, whichever device is current."""
+import contextlib
+import importlib
+
+import pytest
+
+grouped = importlib.import_module("3deecelltracker_amd.grouped")
+gradients = importlib.import_module("3deecelltracker_amd.gradients")
+
+
+class Device:
+    def __init__(self, index):
+        self.index = index
+
+
+class Torch:
+    """Two devices; `captured` is the one whose current stream is being captured"""
+    current, captured = 0, 0
+    int32 = "int32"
+
+    class Tensor:
+        pass
+
+    def __init__(self):
+        outer = self
+
+        class C:
+            _cuda_getDevice = staticmethod(lambda: outer.current)
+            _cuda_isCurrentStreamCapturing = staticmethod(lambda: outer.current == outer.captured)
+
+        @contextlib.contextmanager
+        def device(d):
+            before, outer.current = outer.current, d.index
+            yield
+            outer.current = before
+
+        class Cuda:
+            is_current_stream_capturing = C._cuda_isCurrentStreamCapturing
+        Cuda.device = staticmethod(device)
+        self._C, self.cuda = C, Cuda
+
+    def tensor(self, values, **kw):
+        class Uploaded:
+            to = staticmethod(lambda *a, **k: list(values))
+        return Uploaded()
+
+
+@pytest.mark.parametrize("current", [0, 1])
+@pytest.mark.parametrize("device", [0, 1])
+def test_offsets_on_the_host(monkeypatch, current, device):
+    t = Torch()
+    t.current = current
+    monkeypatch.setattr(grouped, "_env", lambda: (t, {}, None))
+    if device == t.captured:
+        with pytest.raises(ValueError, match="captured"):
+            grouped.offsets_device([0, 2, 3], 2, 3, Device(device))
+    else:
+        assert grouped.offsets_device([0, 2, 3], 2, 3, Device(device)) == [0, 2, 3]
+    assert t.current == current
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_a_gradient_set(monkeypatch, current):
+    t = Torch()
+    t.current = current
+    monkeypatch.setattr(gradients, "_env", lambda: (t, {}, None))
+    monkeypatch.setattr(gradients, "_checked", lambda g, o: ([], [], Device(0)))
+    with pytest.raises(ValueError, match="capture"):
+        gradients.GradientSet([])
