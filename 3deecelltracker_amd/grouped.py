@@ -82,7 +82,7 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
         raise ValueError(f"offsets: must rise from 0 to at most {rows} rows")
     if _capturing(t, device):
         raise ValueError("offsets: numbers on the host cannot be uploaded while a graph is captured; pass an int32 tensor on the device")
-    return t.tensor(host, dtype=t.int32).to(device)
+    return t.tensor(host, dtype=t.int32, pin_memory=True).to(device, non_blocking=True)      # (from pageable memory the copy would wait for the stream)
 
 
 def _as_is(t, a, groups, n, device):

@@ -1,0 +1,31 @@
+"""Grouped products: what a call does beside its numbers (waiting, refusals, sizes)."""
+import importlib
+
+import numpy as np
+import pytest
+
+grouped = importlib.import_module("3deecelltracker_amd.grouped")
+gradients = importlib.import_module("3deecelltracker_amd.gradients")
+_lib = importlib.import_module("3deecelltracker_amd._lib")
+
+
+@pytest.mark.gpu
+def test_offsets_on_the_host_do_not_wait_for_the_stream():
+    """Calls return while work that was enqueued before them still runs, and every one has its own offsets"""
+    import torch as t
+    g = t.Generator(device="cuda").manual_seed(1)
+    x, w = t.randn(60, 32, device="cuda", generator=g), t.randn(3, 32, 16, device="cuda", generator=g)
+    splits = [[0, a, b, 60] for a, b in ((10, 20), (0, 60), (30, 31), (60, 60), (5, 50))]
+    want = [grouped.product(x, w, t.tensor(o, dtype=t.int32, device="cuda")) for o in splits]
+    grouped.product(x, w, splits[0])                       # (the pinned memory is there)
+    big = t.randn(8192, 8192, device="cuda")
+    big @ big
+    t.cuda.synchronize()
+    for _ in range(20):
+        big = (big @ big) * 1e-4                           # more than 100 ms of work
+    busy = t.cuda.Event()
+    busy.record()
+    got = [grouped.product(x, w, o) for o in splits]
+    assert not busy.query()
+    t.cuda.synchronize()
+    assert all(t.equal(a, b) for a, b in zip(got, want))
