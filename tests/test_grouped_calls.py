@@ -29,3 +29,17 @@ def test_offsets_on_the_host_do_not_wait_for_the_stream():
     assert not busy.query()
     t.cuda.synchronize()
     assert all(t.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_scale_and_shift_that_require_grad_are_refused():
+    import torch as t
+    x, w = t.randn(10, 8, device="cuda"), t.randn(2, 8, 6, device="cuda")
+    off, plain = [0, 4, 10], t.ones(2, 6, device="cuda")
+    for learned in (t.ones(2, 6, device="cuda", requires_grad=True), t.ones(6, device="cuda", requires_grad=True), t.ones(2, 12, device="cuda", requires_grad=True)[:, ::2]):
+        for kw in (dict(scale=learned), dict(shift=learned), dict(scale=learned, shift=plain), dict(scale=plain, shift=learned)):
+            with pytest.raises(ValueError, match="requires grad"):
+                grouped.product(x, w, off, **kw)
+            with t.no_grad():
+                y = grouped.product(x, w, off, **kw)
+            assert t.equal(y, grouped.product(x, w, off, **{k: v.detach() for k, v in kw.items()})) and not y.requires_grad
