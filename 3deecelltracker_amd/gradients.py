@@ -11,7 +11,7 @@ import ctypes as C
 import math
 
 from . import _dev, _lib
-from .grouped import _capturing, _env, _on_device
+from .grouped import _capturing, _env, _no_grad, _on_device
 
 _captured: list = []          # the tables that a graph reads: it may be replayed after its set is gone (40 bytes a tensor each)
 
@@ -42,6 +42,7 @@ def _checked(grads, out):
             device = a.device if device is None else device
             if a.device != device:
                 raise ValueError(f"gradient {i}: is on {a.device}, others are on {device}")
+            _no_grad(t, f"gradient {i}", a, ", but norm and clip are not part of torch's graph: pass it detached")
             if a.numel() and not _dense(a):
                 raise ValueError(f"gradient {i}: shape {tuple(a.shape)} with strides {tuple(a.stride())} leaves gaps or overlaps itself")
         if g is not o and (g.dtype != o.dtype or g.shape != o.shape or (g.numel() > 1 and [s for n, s in zip(g.shape, g.stride()) if n > 1] !=

@@ -42,12 +42,12 @@ def _check_tensor(t, types, name, a, dims, dtype, device):
             raise ValueError(f"{name}: values of type {a.dtype} are not supported (float32, bfloat16, float16)")
     if device is not None and a.device != device:
         raise ValueError(f"{name}: is on {a.device}, the other tensors are on {device}")
-    _no_grad(t, name, a, ": pass {name}.detach() and use product_grad")
+    _no_grad(t, name, a, ", but this product is not part of torch's graph: pass {name}.detach() and use product_grad")
 
 
 def _no_grad(t, name, a, instead):
     if a.requires_grad and t.is_grad_enabled():
-        raise ValueError(f"{name}: requires grad, but this product is not part of torch's graph{instead.format(name=name)}")
+        raise ValueError(f"{name}: requires grad{instead.format(name=name)}")
 
 
 def _row_stride(name, rows, cols, row_stride, col_stride):
@@ -101,7 +101,7 @@ def _affine(name, a, groups, n, device):
         raise ValueError(f"{name}: expected a float32 tensor [{n}] or [{groups}, {n}] on {device}")
     if a.shape[-1] != n or (a.dim() == 2 and a.shape[0] not in (1, groups)):
         raise ValueError(f"{name}: shape {tuple(a.shape)} does not fit {groups} groups of {n} columns")
-    _no_grad(t, name, a, ", and its epilogue has no gradient: apply a {name} that is learned outside, or pass {name}.detach()")
+    _no_grad(t, name, a, ", but the product has no gradient for it: apply a {name} that is learned outside, or pass {name}.detach()")
     a = a.contiguous()
     return a, n if a.dim() == 2 and a.shape[0] == groups and groups > 1 else 0
 

@@ -43,3 +43,20 @@ def test_scale_and_shift_that_require_grad_are_refused():
             with t.no_grad():
                 y = grouped.product(x, w, off, **kw)
             assert t.equal(y, grouped.product(x, w, off, **{k: v.detach() for k, v in kw.items()})) and not y.requires_grad
+
+
+@pytest.mark.gpu
+def test_gradients_that_require_grad_are_refused():
+    """Of a backward pass with create_graph: scaled behind torch's back, a second backward pass would use what they are no longer"""
+    import torch as t
+    p = t.ones(50, device="cuda", requires_grad=True)
+    grad, = t.autograd.grad((p * p * p).sum(), p, create_graph=True)
+    for call in (lambda: gradients.clip_by_global_norm([grad], 1.0), lambda: gradients.GradientSet([grad.detach()], out=[p]), lambda: gradients.GradientSet([p])):
+        with pytest.raises(ValueError, match="requires grad"):
+            call()
+    assert bool((grad == 3).all()) and bool((p == 1).all())
+    out, norm = gradients.clip_by_global_norm([grad.detach()], 1.0, out=[t.empty(50, device="cuda")])
+    assert abs(float(norm) - 3 * 50 ** 0.5) <= 22 * 2.0 ** -23 and float(gradients.GradientSet([p.detach()]).norm()) > 7
+    with t.no_grad():
+        gradients.GradientSet([p]).clip(1.0)
+    assert bool((p < 1).all())
