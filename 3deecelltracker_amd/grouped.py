@@ -178,8 +178,9 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
         if tuple(out.shape) != (rows, n):
             raise ValueError(f"out: shape {tuple(out.shape)}, expected {(rows, n)}")
         ldy = _row_stride("out", rows, n, *out.stride())
-        if _overlap(out, x) or _overlap(out, w):
-            raise ValueError("out: overlaps x or w")
+        for name, a in (("x", x), ("w", w), ("the offsets", off), ("scale", sc), ("shift", sh)):
+            if a is not None and _overlap(out, a):
+                raise ValueError(f"out: overlaps {name}")
     rc = _on_device(t, device, L.ct_grouped_product, types[xt], types[dtype], x.data_ptr(), ldx, rows, k, w.data_ptr(), group_stride, ldw, flip, n,
                     off.data_ptr(), g, sc if sc is None else sc.data_ptr(), sh if sh is None else sh.data_ptr(), stride, slope, fill, out.data_ptr(), ldy)
     if rc:

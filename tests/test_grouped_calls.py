@@ -60,3 +60,24 @@ def test_gradients_that_require_grad_are_refused():
     with t.no_grad():
         gradients.GradientSet([p]).clip(1.0)
     assert bool((p < 1).all())
+
+
+@pytest.mark.gpu
+def test_a_result_over_one_of_its_operands_is_refused():
+    """All of them views of one buffer: of each pair, the last value of one is the first of the other"""
+    import torch as t
+    buf = t.zeros(400, device="cuda")
+    x, w, off = buf[:80].view(10, 8), buf[80:176].view(2, 8, 6), t.tensor([0, 4, 10], dtype=t.int32, device="cuda")
+    out = buf[200:260].view(10, 6)
+    inside = buf[259:262].view(t.int32)
+    inside.copy_(off)
+    ones = t.ones(6, device="cuda")
+    for name, call in {"offsets": lambda: grouped.product(x, w, inside, out=out), "scale": lambda: grouped.product(x, w, off, scale=buf[195:201], out=out),
+                       "shift": lambda: grouped.product(x, w, off, scale=ones, shift=buf[259:265], out=out),
+                       "x": lambda: grouped.product(buf[121:201].view(10, 8), w, off, out=out), "w": lambda: grouped.product(x, buf[259:355].view(2, 8, 6), off, out=out)}.items():
+        with pytest.raises(ValueError, match=name):
+            call()
+    inside = buf[260:263].view(t.int32)
+    inside.copy_(off)
+    buf[190:196] = 1.0
+    assert grouped.product(x, w, inside, scale=buf[194:200], shift=buf[263:269], out=out) is out       # end to end is fine
