@@ -49,6 +49,8 @@ struct FF { typedef float S; };
 // ------------------------------------------------------------------------------------------------
 struct Slot { int group, begin, end, row; };        // row: first row of the tile (< end); group == G: rows behind the last group; group < 0: nothing
 
+// ceil(n / step); n up to 2^31 - 1 (n + step may pass it)
+__device__ __forceinline__ int pieces(int n, int step) { return (int)(((uint32_t)n + (uint32_t)(step - 1)) / (uint32_t)step); }
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Which `step` rows of which group tile `idx` stands for: groups are cut into ceil(rows / step) tiles each, numbered in order.  Every wave counts
@@ -64,7 +66,7 @@ __device__ __forceinline__ Slot find_slot(const int32_t* __restrict__ off, int G
             b = clampi(off[g], 0, rows);
             e = g < G ? clampi(off[g + 1], b, rows) : tail ? rows : b;
         }
-        const int tiles = (e - b + step - 1) / step;
+        const int tiles = pieces(e - b, step);
         int sum = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const int v = __shfl_up(sum, d); if (lane >= d) sum += v; }
@@ -377,9 +379,9 @@ struct Core {
 #pragma unroll
                 for (int j = 0; j < SM; ++j) total[i][j] = acc[i][j];
         }
-        const int stages = (end - begin + BK - 1) / BK;
+        const int stages = pieces(end - begin, BK);
         const int full = WAY == EDGE ? stages : (end - begin) / BK;             // stages all of whose steps count; one more may follow
-        auto from = [&](int t) { const int c = begin + t * BK; return WAY == EDGE || c + BK <= extent ? c : extent - BK; };
+        auto from = [&](int t) { const int c = begin + t * BK; return WAY == EDGE || c <= extent - BK ? c : extent - BK; };
         auto pa = [&](int t) { return A + (ACC ? (int64_t)from(t) : (int64_t)from(t) * lda); };
         auto pb = [&](int i, int t) { return B(i) + (BCC ? (int64_t)from(t) : (int64_t)from(t) * ldb); };
         auto fold = [&] {
@@ -635,7 +637,7 @@ __device__ __forceinline__ int2 parts_of(const int32_t* __restrict__ off, int ro
     const int lane = threadIdx.x & 63;
     int before = 0, own = 0;
     for (int h = lane; h <= g; h += 64) {
-        const int b = clampi(off[h], 0, rows), n = (clampi(off[h + 1], b, rows) - b + step - 1) / step;
+        const int b = clampi(off[h], 0, rows), n = pieces(clampi(off[h + 1], b, rows) - b, step);
         if (h < g) before += n; else own = n;
     }
 #pragma unroll
@@ -681,6 +683,7 @@ __global__ __launch_bounds__(ShX::THREADS) void grad_kernel(const ProductP x, co
 
 constexpr int64_t kMaxBlocks = (1 << 22) - 1;               // a grid has fewer than 2^32 work items, a workgroup up to 512
 constexpr int64_t kMaxStride = 1 << 22;                     // a tile's offsets fit 32 bits: 256 rows of 2^22 values
+constexpr int kMaxWidth = 1 << 30;                          // a width and a tile's fit 32 bits
 constexpr int64_t kCus = 256;
 constexpr int kMaxGroups = 1 << 16;                         // every workgroup looks its group up among them, 64 at a time
 
@@ -773,7 +776,7 @@ template <int BK> using AnyK = Shape<32, 32, BK, 1, 1, 8, 2, EDGE>;
 //   any      AnyK    2 x 3181 x 16 fp32, 3 groups      37 : 138 (Any)
 template <typename TT, bool WT, Way WAY>
 int product_pick(const ProductP& p, hipStream_t st) {
-    const int64_t mean = (p.rows + p.G - 1) / p.G, r = p.rows + p.G * 32;       // (a group's last tile is half full on average)
+    const int64_t mean = ((int64_t)p.rows + p.G - 1) / p.G, r = (int64_t)p.rows + p.G * 32;       // (a group's last tile is half full on average)
     const int k = p.K, n = WT ? 1 << 30 : p.N;              // what the tile must not exceed: rows of w may be repeated, columns may not
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2) {
         const int64_t t128 = tiles(r, p.N, 128, 128), t64 = tiles(r, p.N, 64, 64);
@@ -799,7 +802,7 @@ int product_pick(const ProductP& p, hipStream_t st) {
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
         const int64_t t64 = tiles(r, p.N, 64, 64);
-        if (k >= 128 && n >= 32 && tiles(p.rows + p.G * 32, p.N, 16, 32) < kCus) return launch<TT, WT, F16k>(p, st);
+        if (k >= 128 && n >= 32 && tiles(r, p.N, 16, 32) < kCus) return launch<TT, WT, F16k>(p, st);
         if (mean <= 16 && k >= 128 && n >= 64) return launch<TT, WT, F16>(p, st);
         if (mean >= 96 && k >= 32 && p.N >= 128 && tiles(r, p.N, 128, 128) >= 2 * kCus) return launch<TT, WT, F128>(p, st);
         if (k >= 64 && n >= 64 && t64 < 2 * kCus && t64 >= kCus) return launch<TT, WT, F32>(p, st);
@@ -852,7 +855,7 @@ int dw_pick(const DwP& p, hipStream_t st) {
 // groups 12.4 apart, 8.3 together; the worst found is 300 x 128 x 1000 fp32 in 40 groups, 22.5 and 24.6, with 2.2 us less on the host); x: dx as a product (its K is the width of dy, its N the width of x)
 template <typename TT, bool WT, Way WAY>
 int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
-    const int64_t mean = (x.rows + x.G - 1) / x.G, r = x.rows + x.G * 32;
+    const int64_t mean = ((int64_t)x.rows + x.G - 1) / x.G, r = (int64_t)x.rows + x.G * 32;
     auto sum = [&](int t) { return tiles(r, x.N, t, t) + w.G * tiles(w.K, w.N, t, t); };
     const int least = w.part ? 0 : w.K < w.N ? w.K : w.N;   // both widths bound a tile of dw
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2)
@@ -918,7 +921,7 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0) return CT_EINVAL;
     if (rows == 0) return CT_OK;
     if (!offsets || !y || !x || !w || ldy < N || ldx < K || ldw < (w_transposed ? K : N) || w_group_stride < 0 || affine_stride < 0) return CT_EINVAL;
-    if (ldx > kMaxStride || ldw > kMaxStride || G > kMaxGroups) return CT_ESHAPE;
+    if (ldx > kMaxStride || ldw > kMaxStride || G > kMaxGroups || K > kMaxWidth || N > kMaxWidth) return CT_ESHAPE;
     const ProductP p{x, ldx, rows, K, w, w_group_stride, ldw, N, offsets, G, scale, shift, affine_stride, slope, fill_tail != 0, out_type == CT_F32, y, ldy, 0, 0, 0, 0};
     return product_any(type, p, w_transposed != 0, (hipStream_t)stream);
 }
@@ -935,7 +938,7 @@ int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0 || !offsets) return CT_EINVAL;
     if ((rows > 0 && !dy) || lddy < N || (dw && ((rows > 0 && !x) || ldx < K || lddw < N || dw_group_stride < (int64_t)(K - 1) * lddw + N))) return CT_EINVAL;
     if (dx && ((rows > 0 && !w) || ldw < (w_transposed ? K : N) || w_group_stride < 0 || lddx < K)) return CT_EINVAL;
-    if (G > kMaxGroups || lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
+    if (G > kMaxGroups || K > kMaxWidth || N > kMaxWidth || lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
     hipStream_t st = (hipStream_t)stream;
     const ProductP px{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0, 0};
     const int step = dw && rows > 0 ? part_rows(rows, K, N, G) : 0;

@@ -15,6 +15,7 @@ from typing import Sequence, Union
 
 from . import _dev, _lib
 
+MAX_SIZE = (1 << 31) - 1      # rows, columns: the library's sizes have 32 bits, offsets too
 MAX_GROUPS = 1 << 16          # every workgroup looks its group up among them, 64 at a time
 _ready = None
 
@@ -152,6 +153,8 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
         _check_tensor(t, types, "w", w, 3, xt, device)
     rows, k = x.shape
     g, wk, n, flip, ldw, group_stride = _weights("w", w, transposed)
+    if rows > MAX_SIZE or k > MAX_SIZE or n > MAX_SIZE:
+        raise ValueError(f"x {tuple(x.shape)}, w {tuple(w.shape)}: sizes above {MAX_SIZE} are not supported")
     if wk != k:
         raise ValueError(f"x has {k} columns, the weight blocks have {wk} rows")
     ldx = _row_stride("x", rows, k, *x.stride())
@@ -202,6 +205,8 @@ def product_grad(dy, x, w, offsets, *, need_x: bool = True, need_w: bool = True,
         _check_tensor(t, types, "dy", dy, 2, xt, device)
     rows, k = x.shape
     g, wk, n, flip, ldw, group_stride = _weights("w", w, False)
+    if rows > MAX_SIZE or k > MAX_SIZE or n > MAX_SIZE:
+        raise ValueError(f"x {tuple(x.shape)}, w {tuple(w.shape)}: sizes above {MAX_SIZE} are not supported")
     if wk != k or dy.shape != (rows, n):
         raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and w {tuple(w.shape)} do not fit each other")
     ldx, lddy = _row_stride("x", rows, k, *x.stride()), _row_stride("dy", rows, n, *dy.stride())

@@ -310,9 +310,9 @@ int ct_trim_mean(const double* stack, int k, int n3, double cut, double* out, ct
  * y [dev] `out_type` (= type, or CT_F32) [rows][N], row stride ldy; the last index is contiguous everywhere, strides count values, any alignment of a value.
  * offsets [dev] int32 [G + 1], rising from 0 (offsets that do not are clamped: no access outside the tensors, but rows without a defined value).
  * scale, shift [dev] fp32 [G][N] with group stride affine_stride (0: one row for all groups), either may be NULL; slope 1: no activation.
- * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap x or w.  Sums are 32-bit, fp32
+ * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap an operand.  Sums are 32-bit, fp32
  * products exact; their order depends on the sizes alone.
- * CT_ESHAPE: a row stride above 2^22 values, more than 2^16 groups, or more than 2^22 tiles (of at least 16 x 32 values).                   */
+ * CT_ESHAPE: a row stride above 2^22 values, a width above 2^30, more than 2^16 groups, or more than 2^22 tiles (of at least 16 x 32 values). */
 int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
                        int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
                        float slope, int fill_tail, void* y, int64_t ldy, ct_stream_t stream);

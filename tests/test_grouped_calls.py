@@ -81,3 +81,45 @@ def test_a_result_over_one_of_its_operands_is_refused():
     inside.copy_(off)
     buf[190:196] = 1.0
     assert grouped.product(x, w, inside, scale=buf[194:200], shift=buf[263:269], out=out) is out       # end to end is fine
+
+
+def test_the_abi_refuses_widths_whose_tiles_pass_32_bits():
+    if not _lib.LIB_PATH.exists():
+        importlib.import_module("__graft_entry__").build()
+    L = _lib.lib()
+    wide = 2 ** 31 - 1
+    assert L.ct_grouped_product(0, 0, 64, 8, 4, 8, 64, 0, 8, 1, wide, 64, 2, None, None, 0, 1.0, 1, 64, wide, None) == _lib.CT_ESHAPE
+    # dx alone: neither x nor w bounds the width of x where w is stored the other way round
+    assert L.ct_grouped_product_grad(0, 0, 64, 8, None, wide, 4, wide, 64, 0, 8, 0, 8, 64, 2, 64, wide, None, 0, 0, None, 0, None) == _lib.CT_ESHAPE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [1, 2, 3])
+def test_sums_over_as_many_rows_as_32_bits_count(groups):
+    """2^31 - 1 rows of one column: whole numbers at the ends and at the borders, so every sum is exact"""
+    import torch as t
+    rows = 2 ** 31 - 1
+    offsets = {1: [0, rows], 2: [0, 2 ** 30 + 7, rows], 3: [0, 5, 5, rows]}[groups]
+    x, dy = t.zeros(rows, 1, dtype=t.bfloat16, device="cuda"), t.zeros(rows, 1, dtype=t.bfloat16, device="cuda")
+    places = sorted({0, 1, 4, 5, 6, 2 ** 22, 2 ** 30, 2 ** 30 + 6, 2 ** 30 + 7, rows - 65, rows - 64, rows - 2, rows - 1})
+    for i, p in enumerate(places):
+        x[p] = 1.0 + i
+        dy[p] = 2.0
+    w = t.zeros(groups, 1, 1, dtype=t.bfloat16, device="cuda")
+    dw = grouped.product_grad(dy, x, w, offsets, need_x=False, out_dtype=t.float32)[1]
+    want = [sum(2.0 * (1 + i) for i, p in enumerate(places) if a <= p < b) for a, b in zip(offsets, offsets[1:])]
+    assert dw[:, 0, 0].tolist() == want
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused():
+    import torch as t
+    x = t.empty(2 ** 32 + 10, 1, dtype=t.bfloat16, device="cuda")
+    w = t.zeros(1, 1, 1, dtype=t.bfloat16, device="cuda")
+    wide = x[: 2 ** 31 + 5].view(1, 1, 2 ** 31 + 5)
+    with pytest.raises(ValueError, match="sizes above"):
+        grouped.product(x, w, [0, 10])
+    with pytest.raises(ValueError, match="sizes above"):
+        grouped.product(w[0], wide, [0, 1])
+    with pytest.raises(ValueError, match="sizes above"):
+        grouped.product_grad(x, x, w, [0, 10], need_x=False)
