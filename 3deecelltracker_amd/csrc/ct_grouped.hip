@@ -170,9 +170,10 @@ struct Stage {
 // Sources have to be whole pieces (the address a multiple of 4 bytes); rows past the operand take the last one (their results are not stored).
 // The instruction is written out because the compiler's own form makes it wait for all such loads before any read of LDS; Core waits for them.
 // A load does not wait for a base that a v_readfirstlane has just written: that takes five wait states (s_mov and s_nop 3), which the compiler counts for
-// its own loads only; scripts/check_sgpr_waits.py holds the built code to it.
+// its own loads only; scripts/check_sgpr_waits.py holds the built code to it.  m0 is reserved, so a clobber of it means nothing to the compiler: it sets m0
+// itself right before an instruction of its own that reads it, of which these kernels have none (a test counts them).
 __device__ __forceinline__ void direct16(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(voff), "s"(base) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(voff), "s"(base) : "memory");
 }
 template <typename S, bool CC, int E, int BK, int NT>
 struct Direct {
