@@ -289,9 +289,11 @@ struct Core {
     static constexpr int LDS_BYTES = NB * STAGE_BYTES > SUM_BYTES ? NB * STAGE_BYTES : SUM_BYTES;
     static_assert(WAY == DIRECT || NB == 2, "registers hold one stage");
     // fp32 sums of one wave run over at most kChain steps and are then added to the total: a long chain loses a bit for every fourfold length (7542 x 2809 x
-    // 708: 3.9e-7 of the norm, 9.3e-7 as one chain).  Not where waves share a sum: theirs are a quarter as long (4096 steps: 5.7e-7; 4.1e-7 with it, 5 to 15 % slower)
-    static constexpr int kChain = 512;
-    static constexpr bool FOLD = !H && WK == 1;
+    // 708: 3.9e-7 of the norm, 9.3e-7 as one chain; 2^20 rows in four chains 9.2e-6, 8.4e-7 folded, and a hundred times that for values of one sign).
+    // Waves that share a sum fold later, theirs is a quarter or an eighth of it.  A sum that is never folded has no total to carry: a loop of its own.
+    // 16-bit operands carry no more than 11 bits: their sums stay one chain of 32 bits (the totals of 256 x 256 tiles would not fit the registers).
+    static constexpr int kChain = WK == 1 ? 512 : 2048, kFold = kChain / PK;
+    static constexpr bool FOLD = !H;
     typedef typename std::conditional<H, s16x8, f32x4>::type Frag;
     f32x4 acc[SN][SM];
 
@@ -372,39 +374,42 @@ struct Core {
         int m0, n0, kz;
         place(m0, n0, kz);
         ra.init(m0, kz * PK); rb.init(n0, kz * PK);
-        f32x4 total[FOLD ? SN : 1][FOLD ? SM : 1];
         clear();
-        if constexpr (FOLD) {
-#pragma unroll
-            for (int i = 0; i < SN; ++i)
-#pragma unroll
-                for (int j = 0; j < SM; ++j) total[i][j] = acc[i][j];
-        }
         const int stages = pieces(end - begin, BK);
         const int full = WAY == EDGE ? stages : (end - begin) / BK;             // stages all of whose steps count; one more may follow
         auto from = [&](int t) { const int c = begin + t * BK; return WAY == EDGE || c <= extent - BK ? c : extent - BK; };
         auto pa = [&](int t) { return A + (ACC ? (int64_t)from(t) : (int64_t)from(t) * lda); };
         auto pb = [&](int i, int t) { return B(i) + (BCC ? (int64_t)from(t) : (int64_t)from(t) * ldb); };
-        auto fold = [&] {
+        // multiplies the stages of one tile: stretch(t, stop) those up to `stop`, rest(t) the others and the last one
+        auto folded = [&](int& t, auto stretch, auto rest) {
             if constexpr (FOLD) {
+                if (full > kFold) {
+                    f32x4 total[SN][SM];
 #pragma unroll
-                for (int i = 0; i < SN; ++i)
+                    for (int i = 0; i < SN; ++i)
 #pragma unroll
-                    for (int j = 0; j < SM; ++j) { total[i][j] += acc[i][j]; acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+                        for (int j = 0; j < SM; ++j) total[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    do {
+                        stretch(t, t + kFold);
+#pragma unroll
+                        for (int i = 0; i < SN; ++i)
+#pragma unroll
+                            for (int j = 0; j < SM; ++j) total[i][j] += acc[i][j];
+                        clear();
+                    } while (full - t > kFold);
+                    rest(t);
+#pragma unroll
+                    for (int i = 0; i < SN; ++i)
+#pragma unroll
+                        for (int j = 0; j < SM; ++j) acc[i][j] += total[i][j];
+                    return;
+                }
             }
+            rest(t);
         };
-        auto step = [&](int t, int u) {
-            multiply<false>(smem + u % NB * STAGE_BYTES, kz, 0, 0);
-            if constexpr (FOLD) if ((t + 1) % (kChain / BK) == 0) fold();
-        };
+        auto step = [&](int u) { multiply<false>(smem + u % NB * STAGE_BYTES, kz, 0, 0); };
         auto last = [&](int t, int u) { multiply<true>(smem + u % NB * STAGE_BYTES, kz, begin + t * BK - from(t), end - from(t)); };
         auto finish = [&](int i) {
-            if constexpr (FOLD) {
-#pragma unroll
-                for (int a = 0; a < SN; ++a)
-#pragma unroll
-                    for (int b = 0; b < SM; ++b) { acc[a][b] += total[a][b]; total[a][b] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-            }
             if constexpr (WK > 1) join(smem, kz);
             done(i);
         };
@@ -432,16 +437,22 @@ struct Core {
 #pragma unroll
             for (int u = 0; u < NB - 1; ++u) if (u < all) issue(u);
             auto sum = [&](int u) {                                             // the stages of one tile, the first of them u
-                for (int t = 0; t < full; ++t, ++u) {
-                    landed(u);
-                    if (u + NB - 1 < all) issue(u + NB - 1);
-                    step(t, u);
-                }
-                if (full < stages) {
-                    landed(u);
-                    if (u + NB - 1 < all) issue(u + NB - 1);
-                    last(full, u);
-                }
+                int t = 0;
+                auto stretch = [&](int& t, int stop) {
+                    for (; t < stop; ++t, ++u) {
+                        landed(u);
+                        if (u + NB - 1 < all) issue(u + NB - 1);
+                        step(u);
+                    }
+                };
+                folded(t, stretch, [&](int& t) {
+                    stretch(t, full);
+                    if (full < stages) {
+                        landed(u);
+                        if (u + NB - 1 < all) issue(u + NB - 1);
+                        last(full, u);
+                    }
+                });
             };
             if constexpr (MANY) {
                 for (int i = 0; i < tiles; ++i) {
@@ -472,13 +483,19 @@ struct Core {
             };
             if (stages > 0) { load(0); store(0); }
             __syncthreads();
-            for (int t = 0; t < full; ++t) {
-                if (t + 1 < stages) load(t + 1);
-                step(t, t);
-                if (t + 1 < stages) store(t + 1);
-                __syncthreads();
-            }
-            if (full < stages) last(full, full);
+            int t = 0;
+            auto stretch = [&](int& t, int stop) {
+                for (; t < stop; ++t) {
+                    if (t + 1 < stages) load(t + 1);
+                    step(t);
+                    if (t + 1 < stages) store(t + 1);
+                    __syncthreads();
+                }
+            };
+            folded(t, stretch, [&](int& t) {
+                stretch(t, full);
+                if (full < stages) last(full, full);
+            });
             finish(0);
         }
     }
