@@ -1,10 +1,13 @@
-"""Grouped products: how far a long sum may be off."""
+"""Grouped products: that every step of a sum counts exactly once, and how far a long sum may be off.
+
+Whole numbers: with operands in -2 .. 2 a sum of c products is a whole number below 4 c, which 32 bits hold exactly up to c = 2^22, in whatever order; a row
+or column that is left out, counted twice or taken from a neighbour shows as a difference of one or more.  Stored in 16 bits it is the exact sum, rounded."""
 import importlib
 
 import pytest
 
 grouped = importlib.import_module("3deecelltracker_amd.grouped")
-from test_grouped import UNIT
+from test_grouped import CASES, TYPES, UNIT, _offsets
 
 # what a wave adds up before it joins the total, and how many waves share a sum at least where it is that much
 CHAIN, SHARED = 2048, 4
@@ -27,3 +30,44 @@ def test_a_long_sum_is_not_one_chain(case):
         got = grouped.product(t.ones(rows, n, device="cuda"), t.full((1, n, cols), third, device="cuda"), [0, rows])
     off = float((got.double() / (third * n) - 1).abs().max())
     assert off <= (CHAIN + n / (CHAIN * SHARED) + 16) * UNIT
+
+
+def _whole(shape, seed, dtype):
+    import torch as t
+    g = t.Generator(device="cuda").manual_seed(seed)
+    return t.randint(-2, 3, shape, generator=g, device="cuda").to(getattr(t, dtype))
+
+
+def _groups(counts):
+    start = 0
+    for g, c in enumerate(counts):
+        yield g, slice(start, start + c)
+        start += c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts,k,n,tail", CASES, ids=lambda v: str(v)[:24])
+def test_every_step_counts_once(dtype, counts, k, n, tail):
+    import torch as t
+    rows, groups = sum(counts) + tail, len(counts)
+    x, w, dy = _whole((rows, k), 1, dtype), _whole((groups, k, n), 2, dtype), _whole((rows, n), 3, dtype)
+    if tail:
+        x[-tail:] = float("nan"); dy[-tail:] = float("nan")
+    off = _offsets(counts)
+    y, dx, dw = t.zeros(rows, n, dtype=t.float64, device="cuda"), t.zeros(rows, k, dtype=t.float64, device="cuda"), t.zeros(groups, k, n, dtype=t.float64, device="cuda")
+    for g, part in _groups(counts):
+        xs, ws, ds = x[part].double(), w[g].double(), dy[part].double()
+        y[part] = xs @ ws
+        dx[part] = ds @ ws.T.contiguous()
+        dw[g] = xs.T.contiguous() @ ds
+    stored = x.dtype
+    wt = w.transpose(1, 2).contiguous()
+    for got in (grouped.product(x, w, off, out_dtype=t.float32), grouped.product(x, wt, off, transposed=True, out_dtype=t.float32)):
+        assert t.equal(got.double(), y)
+    assert t.equal(grouped.product(x, w, off), y.to(stored))
+    both = grouped.product_grad(dy, x, w, off, out_dtype=t.float32)
+    assert t.equal(both[0], dx.to(stored)) and t.equal(both[1].double(), dw)
+    assert t.equal(grouped.product_grad(dy, x, wt.transpose(1, 2), off)[0], dx.to(stored))
+    assert t.equal(grouped.product_grad(dy, x, w, off, need_w=False)[0], dx.to(stored))
+    assert t.equal(grouped.product_grad(dy, x, w, off, need_x=False)[1], dw.to(stored))
