@@ -847,14 +847,14 @@ int dw_pick(const DwP& p, hipStream_t st) {
     const int r = p.rows, k = p.K, n = p.N;
     if (p.part) {
         int rc;
-        if (WAY != EDGE && sizeof(typename TT::S) == 2 && k >= 64 && n >= 64) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 2, T64<WAY>, Any>, true>(p, st);
+        if (sizeof(typename TT::S) == 2 && k >= 64 && n >= 64) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 2, T64<WAY>, Any>, true>(p, st);
         else if (sizeof(typename TT::S) == 4 && k >= 32 && n >= 32) rc = launch<TT, std::conditional_t<sizeof(typename TT::S) == 4, F32s, Any>, true>(p, st);
         else rc = launch<TT, Any, true>(p, st);
         if (rc != CT_OK) return rc;
         hipLaunchKernelGGL((join_kernel<typename TT::S>), dim3((unsigned)(p.G * ((p.K * p.N + 255) / 256))), dim3(256), 0, st, p);
         return (int)hipGetLastError();
     }
-    if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
+    if constexpr (sizeof(typename TT::S) == 2) {
         if constexpr (WAY == DIRECT)
             if (r >= 64 && k >= 256 && n >= 256 && p.G * tiles(k, n, 256, 256) >= kCus) return launch<TT, T256<WAY>>(p, st);
         if (r >= 64 && k >= 128 && n >= 128 && p.G * tiles(k, n, 128, 128) >= 160) return launch<TT, T128<WAY>>(p, st);
@@ -878,7 +878,7 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     const int least = w.part ? 0 : w.K < w.N ? w.K : w.N;   // both widths bound a tile of dw
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2)
         if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return launch<TT, WT, T256<WAY>, T256<WAY>>(x, w, st);
-    if constexpr (WAY != EDGE && sizeof(typename TT::S) == 2) {
+    if constexpr (sizeof(typename TT::S) == 2) {
         if (mean >= 96 && least >= 128 && sum(128) >= kCus) return launch<TT, WT, T128<WAY>, T128<WAY>>(x, w, st);
         if (x.rows >= 64 && least >= 64) return launch<TT, WT, T64<WAY>, T64<WAY>>(x, w, st);
     }
