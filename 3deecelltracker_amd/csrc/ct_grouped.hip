@@ -885,11 +885,12 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
         if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
         if (x.rows >= 64 && least >= 64) {
-            // 32 x 64 tiles (48 KB: 3 on a CU) where they all run at once and fill it: 2048 x 512 x 512 in 2 groups 23.3 us, 27.4 with 32 x 32;
-            // 500 x 200 x 1000 in 4 groups 16.9, 12.8 with 32 x 32
-            const int64_t n64 = tiles(r, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64);
+            // 32 x 64 tiles (48 KB: 3 on a CU) where they all run at once (with the least tiles that so many rows make; the groups' ends are not known here)
+            // and fill it: 2048 x 512 x 512 in 2 groups (768 tiles) 22.2 us, 26.3 with 32 x 32; 2080 rows (784) 29.3, 27.4 with 32 x 32;
+            // 2048 x 256 x 256 in 16 groups (768) 11.1 and 11.6; 500 x 200 x 1000 in 4 groups 16.9, 12.8 with 32 x 32
+            const int64_t n64 = tiles(r, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64), least64 = tiles(x.rows, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64);
             if (sum(64) >= 2 * kCus && n64 > 4 * kCus) return launch<TT, WT, F64, F64>(x, w, st);
-            if (n64 >= 2 * kCus && n64 <= 3 * kCus + kCus / 8) return launch<TT, WT, F32, F32>(x, w, st);
+            if (n64 >= 2 * kCus && least64 <= 3 * kCus) return launch<TT, WT, F32, F32>(x, w, st);
             return launch<TT, WT, F32s, F32s>(x, w, st);
         }
     }
