@@ -52,7 +52,7 @@ int ct_stream_create_cu_range(int device, int first_cu, int n_cu, ct_stream_t* o
     for (int c = first_cu; c < first_cu + n_cu; ++c) mask[c / 32] |= (1u << (c % 32));
     hipStream_t st;
     e = hipExtStreamCreateWithCUMask(&st, (uint32_t)words, mask);
-    if (e != hipSuccess) return (int)e;
+    if (e != hipSuccess) { (void)hipGetLastError(); return (int)e; }            // (said here: the next launch must not report it again)
     *out = (ct_stream_t)st;
     return CT_OK;
 }
