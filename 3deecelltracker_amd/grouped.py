@@ -188,6 +188,8 @@ def product(x, w, offsets, *, transposed: bool = False, scale=None, shift=None, 
                     off.data_ptr(), g, sc if sc is None else sc.data_ptr(), sh if sh is None else sh.data_ptr(), stride, slope, fill, out.data_ptr(), ldy)
     if rc:
         _lib.check(rc, "ct_grouped_product")
+    if not fill:
+        t.autograd.graph.increment_version(out)               # (a graph that saved `out` learns that it holds other values now)
     return out
 
 

@@ -123,3 +123,18 @@ def test_sizes_past_32_bits_are_refused():
         grouped.product(w[0], wide, [0, 1])
     with pytest.raises(ValueError, match="sizes above"):
         grouped.product_grad(x, x, w, [0, 10], need_x=False)
+
+
+@pytest.mark.gpu
+def test_a_given_result_that_a_graph_has_saved():
+    """As with every operation in place: the backward pass that needs the old values refuses, instead of using the new ones"""
+    import torch as t
+    x, w, off = t.randn(10, 8, device="cuda"), t.randn(2, 8, 6, device="cuda"), t.tensor([0, 4, 10], dtype=t.int32, device="cuda")
+    out, p = t.zeros(10, 6, device="cuda"), t.ones(10, 6, device="cuda", requires_grad=True)
+    grouped.product(x, w, off, out=out)
+    loss = (p * out).sum()
+    grouped.product(x + 1, w, off, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with t.inference_mode():
+        assert grouped.product(x, w, off, out=t.zeros(10, 6, device="cuda")).is_inference()
