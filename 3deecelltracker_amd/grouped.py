@@ -80,7 +80,13 @@ def offsets_device(offsets: Union[Sequence[int], "torch.Tensor"], groups: int, r
         if offsets.dtype is not t.int32 or offsets.dim() != 1 or offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
             raise ValueError(f"offsets: expected a contiguous int32 tensor of {groups + 1} numbers, got {offsets.dtype} {tuple(offsets.shape)}")
         raise ValueError(f"offsets: are on {offsets.device}, the other tensors are on {device}")
-    host = [int(v) for v in (offsets.tolist() if hasattr(offsets, "tolist") else offsets)]
+    given = offsets.tolist() if hasattr(offsets, "tolist") else list(offsets)
+    try:
+        host = [int(v) for v in given]
+    except (TypeError, ValueError, OverflowError):
+        host = None
+    if host is None or host != given:
+        raise ValueError("offsets: must be whole numbers")
     if len(host) != groups + 1:
         raise ValueError(f"offsets: expected {groups + 1} numbers for {groups} groups, got {len(host)}")
     if host[0] != 0 or any(a > b for a, b in zip(host, host[1:])) or host[-1] > rows:

@@ -67,3 +67,21 @@ def test_a_gradient_set(monkeypatch, current):
     monkeypatch.setattr(gradients, "_checked", lambda g, o: ([], [], Device(0)))
     with pytest.raises(ValueError, match="capture"):
         gradients.GradientSet([])
+
+
+@pytest.mark.parametrize("offsets", [[0, 2.5, 10], [0, float("nan"), 10], [0, float("inf"), 10], [0, None, 10], [[0, 2], [2, 10], [10, 10]], [0, "2", 10]], ids=str)
+def test_offsets_that_are_not_whole_numbers(monkeypatch, offsets):
+    """None of them may be rounded in silence"""
+    monkeypatch.setattr(grouped, "_env", lambda: (Torch(), {}, None))
+    with pytest.raises(ValueError, match="whole numbers"):
+        grouped.offsets_device(offsets, 2, 10, Device(1))
+
+
+@pytest.mark.parametrize("offsets", [[0, 2, 10], (0, 2, 10), [0.0, 2.0, 10.0], "int64", "float64"], ids=str)
+def test_offsets_that_are(monkeypatch, offsets):
+    import numpy as np
+    monkeypatch.setattr(grouped, "_env", lambda: (Torch(), {}, None))
+    if isinstance(offsets, str):
+        offsets = np.array([0, 2, 10], dtype=offsets)
+    got = grouped.offsets_device(offsets, 2, 10, Device(1))
+    assert got == [0, 2, 10] and all(type(v) is int for v in got)
