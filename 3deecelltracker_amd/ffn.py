@@ -175,13 +175,14 @@ class FFN:
         if x.ndim != 2 or x.shape[1] != 2 * FFN_FEAT:
             raise ValueError(f"expected input of shape (P, {2 * FFN_FEAT}), got {x.shape}")
         out = np.empty((x.shape[0], 1), dtype=np.float32)
+        handle = self._handle                  # one for all pieces: a training step beside them does not mix two sets of weights in one result
         step = 1 << 18
         for s in range(0, x.shape[0], step):
             xd = _dev.to_dev(x[s:s + step], t.float32, f"cuda:{self._device}")
             rows = xd.shape[0]
             od = _dev.empty((rows,), t.float32, xd.device)
             ws = _dev.workspace(L.ct_ffn_predict_workspace_bytes(rows), xd.device)
-            _lib.check(L.ct_ffn_predict(self._handle, xd.data_ptr(), rows, od.data_ptr(), ws.data_ptr(), ws.numel(),
+            _lib.check(L.ct_ffn_predict(handle, xd.data_ptr(), rows, od.data_ptr(), ws.data_ptr(), ws.numel(),
                                         _dev.stream(xd.device)), "ct_ffn_predict")
             out[s:s + rows, 0] = od.cpu().numpy()
         return out

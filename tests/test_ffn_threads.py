@@ -121,11 +121,16 @@ class Library:
                 assert number in keep.alive, f"handle {number} was destroyed during a call"
                 return 0
         self.ct_ffn_pairgrid = Entry()
+        self.ct_ffn_predict = lambda handle, *rest: self.asked.append(handle._as_parameter_.value) or (self.inside and self.inside()) or 0
+        self.asked = []
 
     def ct_ffn_num_weights(self):
         return 3
 
     def ct_ffn_workspace_bytes(self, n, m):
+        return 16
+
+    def ct_ffn_predict_workspace_bytes(self, rows):
         return 16
 
     def ct_ffn_create(self, w, n, device, out):
@@ -206,3 +211,13 @@ def test_a_model_without_weights_can_be_copied(library):
     for m in (copy.deepcopy(ffn_mod.FFN(device=0)), pickle.loads(pickle.dumps(ffn_mod.FFN(device=0)))):
         m.set_weights_dict({"size": 3})
         assert m._handle is not None and m._device == 0
+
+
+def test_a_prediction_in_pieces_has_one_set_of_weights(library, monkeypatch):
+    import torch
+    monkeypatch.setattr(_dev, "to_dev", lambda a, dtype, device=None: torch.as_tensor(a, dtype=dtype))
+    m = ffn_mod.FFN(device=0)
+    m.set_weights_dict({"size": 3})
+    library.inside = lambda: m.set_weights_dict({"size": 3}) and None      # what a training step on another thread amounts to
+    m.predict(np.zeros(((1 << 18) + 1, 122), np.float32))
+    assert library.asked == [1, 1] and library.alive == {3}
