@@ -1,0 +1,66 @@
+"""Several training steps in a row against the same steps in 64 bits: Adam's moments and their corrections, the moving statistics, weights that the next
+step builds on.
+
+epsilon = 1 keeps Adam's division away from gradients near zero: an update is rate * m / (sqrt(v) + 1), which follows the gradients' errors at most
+one to one.  A gradient is off by at most 2e-3 of its norm (test_ffn_training.py), so is a sum of updates, and so is the next gradient's change
+through weights that moved by a fraction of themselves; twice that is allowed.  Corrections of the wrong step would show as a fourth."""
+import importlib
+
+import numpy as np
+import pytest
+
+ffn_mod = importlib.import_module("3deecelltracker_amd.ffn")
+synth = importlib.import_module("3deecelltracker_amd.synth")
+from test_ffn_training import TOL, _batch, _reference
+
+pytestmark = pytest.mark.gpu
+NAMES = ("w1", "gamma1", "beta1", "w2", "gamma2", "beta2", "w3", "b3")
+
+
+def _flat(w):
+    return {"w1": w["w1"], "gamma1": w["bn1"]["gamma"], "beta1": w["bn1"]["beta"], "w2": w["w2"], "gamma2": w["bn2"]["gamma"], "beta2": w["bn2"]["beta"],
+            "w3": np.reshape(w["w3"], (-1, 1)), "b3": np.reshape(w["b3"], -1)}
+
+
+def _steps(w, batches, rate, b1, b2, eps, clip):
+    """-> (losses, weights, moving statistics) after one update for each batch"""
+    p = {k: np.asarray(v, dtype=np.float64).copy() for k, v in _flat(w).items()}
+    m = {k: np.zeros_like(v) for k, v in p.items()}
+    v = {k: np.zeros_like(a) for k, a in p.items()}
+    moving = {f"{s}{i}": np.asarray(w[f"bn{i}"][s], dtype=np.float64) for i in (1, 2) for s in ("mean", "var")}
+    losses = []
+    for t, (x, y) in enumerate(batches, 1):
+        now = {"w1": p["w1"], "w2": p["w2"], "w3": p["w3"], "b3": p["b3"]}
+        for i in (1, 2):
+            now[f"bn{i}"] = {"gamma": p[f"gamma{i}"], "beta": p[f"beta{i}"], "mean": moving[f"mean{i}"], "var": moving[f"var{i}"]}
+        loss, g, moving = _reference(now, x, y)
+        losses.append(loss)
+        norm = np.sqrt(sum((a ** 2).sum() for a in g.values()))
+        scale = clip / max(norm, clip) if clip else 1.0
+        for k in NAMES:
+            m[k] = b1 * m[k] + (1 - b1) * g[k] * scale
+            v[k] = b2 * v[k] + (1 - b2) * (g[k] * scale) ** 2
+            p[k] -= rate * np.sqrt(1 - b2 ** t) / (1 - b1 ** t) * m[k] / (np.sqrt(v[k]) + eps)
+    return losses, p, moving
+
+
+@pytest.mark.parametrize("clip", [None, 0.05])
+def test_steps_in_a_row(clip):
+    w = synth.make_ffn_weights(seed=4, gain=6.0)
+    batches = [_batch(rows, 20 + rows) for rows in (128, 128, 61, 300, 128)]
+    rate = 0.5 if clip is None else 5.0
+    model = ffn_mod.FFN().set_weights_dict(w)
+    model.compile(learning_rate=rate, epsilon=1.0, global_clipnorm=clip)
+    losses = [model.train_on_batch(x, y) for x, y in batches]
+    want_losses, want, moving = _steps(w, batches, rate, 0.9, 0.999, 1.0, clip)
+    assert np.allclose(losses, want_losses, rtol=0, atol=2 * TOL * max(1.0, max(want_losses)))
+    got, first = _flat(model._training.weights()), _flat(w)
+    for k in NAMES:
+        moved, expected = np.asarray(got[k], dtype=np.float64) - first[k], want[k] - first[k]
+        rounding = 5 * 2.0 ** -24 * np.linalg.norm(want[k])                # the weight that each update is added to
+        assert np.linalg.norm(moved - expected) <= 2 * TOL * np.linalg.norm(expected) + rounding, k
+        assert np.linalg.norm(expected) > 20 * rounding, k
+    after = model._training.weights()
+    for i in (1, 2):
+        for s in ("mean", "var"):
+            assert np.abs(after[f"bn{i}"][s] - moving[f"{s}{i}"]).max() <= 2 * TOL * np.abs(moving[f"{s}{i}"]).max()
