@@ -706,6 +706,7 @@ constexpr int64_t kCus = 256;
 constexpr int kMaxGroups = 1 << 16;                         // every workgroup looks its group up among them, 64 at a time
 
 bool type_ok(int t) { return t == CT_F32 || t == CT_BF16 || t == CT_F16; }
+bool at_value(const void* p, int type) { return ((uintptr_t)p & (type == CT_F32 ? 3 : 1)) == 0; }
 bool words(const void* p, int64_t ld, int64_t more, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size) | (uintptr_t)(more * size)) & 3) == 0; }
 int64_t tiles(int64_t m, int64_t n, int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
@@ -940,6 +941,7 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0) return CT_EINVAL;
     if (rows == 0) return CT_OK;
     if (!offsets || !y || !x || !w || ldy < N || ldx < K || ldw < (w_transposed ? K : N) || w_group_stride < 0 || affine_stride < 0) return CT_EINVAL;
+    if (!at_value(x, type) || !at_value(w, type) || !at_value(y, out_type) || !at_value(offsets, CT_F32) || !at_value(scale, CT_F32) || !at_value(shift, CT_F32)) return CT_EINVAL;
     if (ldx > kMaxStride || ldw > kMaxStride || G > kMaxGroups || K > kMaxWidth || N > kMaxWidth) return CT_ESHAPE;
     const ProductP p{x, ldx, rows, K, w, w_group_stride, ldw, N, offsets, G, scale, shift, affine_stride, slope, fill_tail != 0, out_type == CT_F32, y, ldy, 0, 0, 0, 0};
     return product_any(type, p, w_transposed != 0, (hipStream_t)stream);
@@ -957,6 +959,7 @@ int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy
     if (!type_ok(type) || !(out_type == type || out_type == CT_F32) || rows < 0 || K <= 0 || N <= 0 || G <= 0 || !offsets) return CT_EINVAL;
     if ((rows > 0 && !dy) || lddy < N || (dw && ((rows > 0 && !x) || ldx < K || lddw < N || dw_group_stride < (int64_t)(K - 1) * lddw + N))) return CT_EINVAL;
     if (dx && ((rows > 0 && !w) || ldw < (w_transposed ? K : N) || w_group_stride < 0 || lddx < K)) return CT_EINVAL;
+    if (!at_value(dy, type) || !at_value(offsets, CT_F32) || (dw && (!at_value(x, type) || !at_value(dw, out_type))) || (dx && (!at_value(w, type) || !at_value(dx, type)))) return CT_EINVAL;
     if (G > kMaxGroups || K > kMaxWidth || N > kMaxWidth || lddy > kMaxStride || (dw && ldx > kMaxStride) || (dx && ldw > kMaxStride)) return CT_ESHAPE;
     hipStream_t st = (hipStream_t)stream;
     const ProductP px{dy, lddy, rows, N, w, w_group_stride, ldw, K, offsets, G, nullptr, nullptr, 0, 1.f, 1, type == CT_F32, dx, lddx, 0, 0, 0, 0};

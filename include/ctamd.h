@@ -307,11 +307,12 @@ int ct_trim_mean(const double* stack, int k, int n3, double cut, double* out, ct
  *     y[r][n] = act(scale[g][n] * sum_k x[r][k] w[g][k][n] + shift[g][n]),   act(v) = v >= 0 ? v : slope * v
  * x [dev] `type` [rows][K], row stride ldx; w [dev] `type` [G][K][N], or [G][N][K] with w_transposed (then this is the product's gradient with
  * respect to x: x = dy, K = the layer's width, N = its input's), row stride ldw, group stride w_group_stride (0: one block for all groups);
- * y [dev] `out_type` (= type, or CT_F32) [rows][N], row stride ldy; the last index is contiguous everywhere, strides count values, any alignment of a value.
+ * y [dev] `out_type` (= type, or CT_F32) [rows][N], row stride ldy; the last index is contiguous everywhere, strides count values, any address that is a multiple of a value.
  * offsets [dev] int32 [G + 1], rising from 0 (offsets that do not are clamped: no access outside the tensors, but rows without a defined value).
  * scale, shift [dev] fp32 [G][N] with group stride affine_stride (0: one row for all groups), either may be NULL; slope 1: no activation.
  * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap an operand.  Sums are 32-bit, fp32
- * products exact; their order depends on the sizes alone.
+ * products exact; their order depends on the sizes and on the alignment and layout of x and w, never on values or timing.  fp32 sums are folded every
+ * 512 to 2048 steps of a wave; those of 16-bit operands are single chains (of n values of one sign at most n 2^-24 off).
  * CT_ESHAPE: a row stride above 2^22 values, a width above 2^30, more than 2^16 groups, or more than 2^22 tiles (of at least 16 x 32 values). */
 int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
                        int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
@@ -321,7 +322,8 @@ int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int r
  *     dx[r][k] = sum_n dy[r][n] w[g][k][n]                           [rows][K] of `type`, row stride lddx; zero behind offsets[G]
  *     dw[g][k][n] = sum over the rows r of group g of x[r][k] dy[r][n]    [G][K][N] of `out_type`; zero for a group without rows
  * x, w as above (w_transposed: stored [G][N][K]); dx or dw may be NULL (then w or x is not looked at).  dw: row stride lddw, group stride
- * dw_group_stride (groups must not overlap).  The order of every sum depends on the sizes and on which of the two are asked for.
+ * dw_group_stride (groups must not overlap); dx and dw must overlap nothing.  The order of every sum depends on the sizes, on the alignment and
+ * layout of the operands, and on which of the two are asked for.
  * Workspace [dev], 4-byte aligned: long sums for few weights are made in parts (0 bytes: NULL is fine).                                  */
 size_t ct_grouped_product_grad_workspace_bytes(int type, int rows, int K, int N, int G);
 int ct_grouped_product_grad(int type, int out_type, const void* dy, int64_t lddy, const void* x, int64_t ldx, int rows, int K, const void* w,

@@ -138,3 +138,17 @@ def test_a_given_result_that_a_graph_has_saved():
         loss.backward()
     with t.inference_mode():
         assert grouped.product(x, w, off, out=t.zeros(10, 6, device="cuda")).is_inference()
+
+
+def test_the_abi_refuses_addresses_between_values():
+    """Direct loads take whole words: an fp32 tensor at an address that is no multiple of 4, or 16-bit values at an odd one, is refused, not read"""
+    L = _lib.lib()
+    ok = dict(type=0, out=0, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, sc=None, sh=None, ag=0, slope=1.0, fill=1, y=64, ldy=6, st=None)
+    product = lambda **kw: L.ct_grouped_product(*{**ok, **kw}.values())
+    for kw in (dict(x=66), dict(w=66), dict(y=66), dict(off=66), dict(sc=66), dict(sh=65), dict(type=1, out=1, x=65), dict(type=2, out=2, w=67), dict(type=1, out=1, y=65),
+               dict(type=1, out=0, y=66)):
+        assert product(**kw) == _lib.CT_EINVAL, kw
+    ok2 = dict(type=0, out=0, dy=64, lddy=6, x=64, ldx=8, rows=4, K=8, w=64, wg=48, ldw=6, wt=0, N=6, off=64, G=2, dx=64, lddx=8, dw=64, dwg=48, lddw=6, ws=None, wsb=0, st=None)
+    grad = lambda **kw: L.ct_grouped_product_grad(*{**ok2, **kw}.values())
+    for kw in (dict(dy=66), dict(x=66), dict(w=66), dict(off=66), dict(dx=66), dict(dw=66), dict(type=1, out=1, dy=65), dict(type=1, out=0, dw=66), dict(type=2, out=2, dx=65)):
+        assert grad(**kw) == _lib.CT_EINVAL, kw
