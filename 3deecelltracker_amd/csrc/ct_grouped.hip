@@ -877,26 +877,42 @@ int grad_pick(const ProductP& x, const DwP& w, hipStream_t st) {
     const int64_t mean = ((int64_t)x.rows + x.G - 1) / x.G, r = (int64_t)x.rows + x.G * 32;
     auto sum = [&](int t) { return tiles(r, x.N, t, t) + w.G * tiles(w.K, w.N, t, t); };
     const int least = w.part ? 0 : w.K < w.N ? w.K : w.N;   // both widths bound a tile of dw
+    auto apart = [&] {
+        const int rc = dw_pick<TT, WAY>(w, st);             // (also a sum in parts)
+        return rc == CT_OK ? product_pick<TT, WT, WAY>(x, st) : rc;
+    };
+    // One shape for both, unless it starves one of them, which apart would get tiles of its own:
+    //   long sums in few tiles of dw    16384 x 512 x 512 fp32 in 1 group 1053 us together, 199 apart (16 tiles); 16384 x 1024 x 1024 in 2 groups 623 : 558 (128);
+    //                                   4096 x 1024 x 1024 in 8 groups, shorter sums, 135 : 144; bf16 16384 x 512 x 512 161 : 90 (16), in 8 groups 31 : 35 (128)
+    //   fp32, few tiles of dx           1024 x 1024 x 1024 in 8 groups 79 : 49 (80 tiles, 512 of dw), 1024 x 2048 x 1536 in 8 groups 164 : 132 (160);
+    //                                   1024 x 512 x 512 in 8 groups, small enough for one launch to pay, 15 : 19
+    auto both = [&](auto shape) {
+        typedef decltype(shape) Sh;
+        const int64_t tx = tiles(r, x.N, Sh::BM, Sh::BN), tw = w.G * tiles(w.K, w.N, Sh::BM, Sh::BN);
+        constexpr bool H = sizeof(typename TT::S) == 2;
+        if (mean >= 2048 && tw < (H ? kCus / 4 : kCus * 3 / 4)) return apart();
+        if (!H && Sh::BM >= 64 && tx <= kCus * 5 / 8 && tw >= kCus * 3 / 2 && (int64_t)x.rows * w.K * w.N >= 1 << 28) return apart();
+        return launch<TT, WT, Sh, Sh>(x, w, st);
+    };
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 2)
-        if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return launch<TT, WT, T256<WAY>, T256<WAY>>(x, w, st);
+        if (mean >= 192 && least >= 256 && sum(256) >= 2 * kCus) return both(T256<WAY>{});
     if constexpr (sizeof(typename TT::S) == 2) {
-        if (mean >= 96 && least >= 128 && sum(128) >= kCus) return launch<TT, WT, T128<WAY>, T128<WAY>>(x, w, st);
-        if (x.rows >= 64 && least >= 64) return launch<TT, WT, T64<WAY>, T64<WAY>>(x, w, st);
+        if (mean >= 96 && least >= 128 && sum(128) >= kCus) return both(T128<WAY>{});
+        if (x.rows >= 64 && least >= 64) return both(T64<WAY>{});
     }
     if constexpr (WAY == DIRECT && sizeof(typename TT::S) == 4) {
-        if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return launch<TT, WT, F128, F128>(x, w, st);
+        if (mean >= 96 && least >= 128 && sum(128) >= 2 * kCus) return both(F128{});
         if (x.rows >= 64 && least >= 64) {
             // 32 x 64 tiles (48 KB: 3 on a CU) where they all run at once (with the least tiles that so many rows make; the groups' ends are not known here)
             // and fill it: 2048 x 512 x 512 in 2 groups (768 tiles) 22.2 us, 26.3 with 32 x 32; 2080 rows (784) 29.3, 27.4 with 32 x 32;
             // 2048 x 256 x 256 in 16 groups (768) 11.1 and 11.6; 500 x 200 x 1000 in 4 groups 16.9, 12.8 with 32 x 32
             const int64_t n64 = tiles(r, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64), least64 = tiles(x.rows, x.N, 32, 64) + w.G * tiles(w.K, w.N, 32, 64);
-            if (sum(64) >= 2 * kCus && n64 > 4 * kCus) return launch<TT, WT, F64, F64>(x, w, st);
-            if (n64 >= 2 * kCus && least64 <= 3 * kCus) return launch<TT, WT, F32, F32>(x, w, st);
-            return launch<TT, WT, F32s, F32s>(x, w, st);
+            if (sum(64) >= 2 * kCus && n64 > 4 * kCus) return both(F64{});
+            if (n64 >= 2 * kCus && least64 <= 3 * kCus) return both(F32{});
+            return both(F32s{});
         }
     }
-    const int rc = dw_pick<TT, WAY>(w, st);                 // (also a sum in parts)
-    return rc == CT_OK ? product_pick<TT, WT, WAY>(x, st) : rc;
+    return apart();
 }
 
 // direct loads want addresses that are multiples of 4 bytes (16-bit values: an even stride, and an even width where the last tile is moved back);
