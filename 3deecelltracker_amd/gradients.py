@@ -11,7 +11,7 @@ import ctypes as C
 import math
 
 from . import _dev, _lib
-from .grouped import _capturing, _env, _no_grad, _on_device
+from .grouped import _capturing, _env, _no_grad
 
 _captured: list = []          # the tables that a graph reads: it may be replayed after its set is gone (40 bytes a tensor each)
 
@@ -84,7 +84,7 @@ class GradientSet:
             _env()[0].cuda.current_stream(self._device).synchronize()
 
     def _init(self, grads, out, once=False):
-        t, kinds, L = _env()
+        t, kinds, L = self._t, _, self._lib = _env()
         self.grads, self.out, self._device = _checked(grads, out)
         self._n = len(self.grads)
         if self._device is None:                              # an empty list: its norm is zero, on the current device
@@ -106,38 +106,40 @@ class GradientSet:
 
     def _used_on(self, t, stream):
         """The memory that a call on a stream other than the list's own reads and writes is not handed out again before that stream is through"""
-        with t.cuda.device(self._device):
-            current = t.cuda.current_stream()
-            for a in {id(a): a for a in (self._table, *self.grads, *self.out)}.values():
-                a.record_stream(current)
+        current = t.cuda.current_stream()
+        for a in {id(a): a for a in (self._table, *self.grads, *self.out)}.values():
+            a.record_stream(current)
         self._streams.add(stream)
 
     def _call(self, call, *args):
-        t = _env()[0]
-        stream = t._C._cuda_getCurrentRawStream(self._device.index)
-        if _capturing(t, self._device):
+        t, device = self._t, self._device
+        if t._C._cuda_getDevice() != device.index:
+            with t.cuda.device(device):
+                return self._call(call, *args)
+        stream = t._C._cuda_getCurrentRawStream(device.index)
+        if t._C._cuda_isCurrentStreamCapturing():
             if not self._keeps:
                 _captured.append(self._table)
                 self._keeps = True
         elif stream not in self._streams:
             self._used_on(t, stream)
         # the scalar and the partial sums, new for each call: two streams, or two graphs, share none
-        scalar, ws = t.empty((), dtype=t.float32, device=self._device), t.empty(self._ws, dtype=t.uint8, device=self._device)
-        rc = _on_device(t, self._device, call, self._at, self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws)
+        scalar, ws = t.empty((), dtype=t.float32, device=device), t.empty(self._ws, dtype=t.uint8, device=device)
+        rc = call(self._at, self._n, self._chunks, *args, scalar.data_ptr(), ws.data_ptr(), self._ws, stream)
         if rc:
             _lib.check(rc, call.__name__)
         return scalar
 
     def norm(self):
         """The l2 norm over all values, a float32 scalar on the device (asynchronous)."""
-        return self._call(_env()[2].ct_gradset_norm)
+        return self._call(self._lib.ct_gradset_norm)
 
     def clip(self, clip_norm: float):
         """Scale the gradients to at most `clip_norm` (into `out`, or in place) -> their norm before that, a float32 scalar on the device."""
         clip_norm = float(clip_norm)
         if not (clip_norm > 0.0 and math.isfinite(clip_norm)):
             raise ValueError(f"clip_norm must be positive and finite, got {clip_norm}")
-        return self._call(_env()[2].ct_gradset_clip, clip_norm)
+        return self._call(self._lib.ct_gradset_clip, clip_norm)
 
 
 def clip_by_global_norm(grads, clip_norm: float, out=None):

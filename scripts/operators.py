@@ -4,6 +4,7 @@
     python scripts/operators.py extra                                 what the workloads leave out: dx and dw apart, few rows a group, the group look-up, the norm
                                                                       alone, offsets on the host, the one-use clip, a training step
     python scripts/operators.py run [--calls N] [--only NAME,NAME]    N passes of each on the kernels, for a profiler
+    python scripts/operators.py counters FILE                         rocprofv3's counter_collection.csv of such a run -> the mean of each counter by kernel
 
 The files operators_*.txt and operators_*.csv under profiles/ are what it printed, or what rocprofv3 wrote beside it."""
 from __future__ import annotations
@@ -135,15 +136,30 @@ def extra(o, args):
         say(f"FFN.train_on_batch, {rows} pairs on the device", passes(lambda: model.train_on_batch(x, y)))
 
 
+def counters(o, args):
+    import csv
+    found = {}
+    for row in csv.DictReader(open(args.file, newline="")):
+        name = row["Kernel_Name"]
+        if any(k in name for k in ("product_kernel", "dw_kernel", "grad_kernel", "join_kernel", "norm_kernel", "clip_kernel")):
+            found.setdefault(name, {}).setdefault(row["Counter_Name"], []).append(float(row["Counter_Value"]))
+    columns = sorted({c for v in found.values() for c in v})
+    out = csv.writer(sys.stdout, lineterminator="\n")
+    out.writerow(["kernel", "calls", *columns])
+    for name, v in found.items():
+        out.writerow([name, max(len(x) for x in v.values()), *(round(sum(v[c]) / len(v[c])) for c in columns)])
+
+
 def main():
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    p.add_argument("what", choices=["times", "extra", "run"])
+    p.add_argument("what", choices=["times", "extra", "run", "counters"])
+    p.add_argument("file", nargs="?")
     p.add_argument("--draw", type=int, default=0)
     p.add_argument("--only", default="")
     p.add_argument("--calls", type=int, default=23)
     args = p.parse_args()
-    o = importlib.import_module("perf.operators")
-    {"times": times, "extra": extra, "run": run}[args.what](o, args)
+    o = importlib.import_module("perf.operators") if args.what != "counters" else None
+    {"counters": counters, "times": times, "extra": extra, "run": run}[args.what](o, args)
 
 
 if __name__ == "__main__":
