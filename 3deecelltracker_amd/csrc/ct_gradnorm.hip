@@ -7,10 +7,10 @@
 // vanishes there, and the partial sums are added in one order that depends on the sizes alone, so a norm repeats bit for bit.
 //
 // Bound by memory, and for small lists by the launches and by loads that wait for each other (measured on MI355X):
-//   * 300 M bf16 values into other tensors: 384 us, 1.8 GB in three passes = 4.7 TB/s where a copy runs at 5.1 (64-bit sums cost nothing beside that:
-//     reading alone goes at 6.1 TB/s with them).  The second pass goes backwards, which saves 1 %.
-//   * 1200 tensors, 9 M values: 20.7 us (8.4 + 11.8); with halving instead of the 64-wide search, tails piece by piece and 2048 workgroups 28.5.
-//   * 9 tensors, 0.56 M values: 10.4 us (3.6 + 4.6 and the call).
+//   * 300 M bf16 values into other tensors: 385 to 397 us, 1.8 GB in three passes = 4.6 TB/s where a copy runs at 5.1 (146 + 238 us; the norm alone, with
+//     nothing being written back beside it, goes at 5.5 TB/s, 64-bit sums and all).  The second pass goes backwards, which saves 1 %.
+//   * 1200 tensors, 9 M values: 19.4 us (8.4 + 11.8); with halving instead of the 64-wide search, tails piece by piece and 2048 workgroups 28.5.
+//   * 9 tensors, 0.56 M values: 10.7 us (3.7 + 4.6 and the call); as a list that is used once 61 us, most of it the host's checks.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -12,16 +12,19 @@
 // What bounds it, and what was chosen for it (measured on MI355X; a copy runs at 5.1 TB/s there, a library product of 8192^3 at 1189 TFLOP/s in bf16
 // and 153 in fp32):
 //   * large groups, 16 bit: the matrix pipe (55 % busy) and, next to it, LDS.  256 x 256 tiles of 8 waves, two 64 KB stages filled by direct loads:
-//     32768 x 4096 x 2048 in 16 uneven groups 560 us = 980 TFLOP/s (542-575 over boxes; 128 x 128 tiles 650), its gradients at 16384 x 2048 x 1536 285 us.
-//   * a few rows a group: the weights, each read once.  16 x 64 tiles, every wave a quarter of a stage's sum: 64 rows of 2048 x 1024 blocks 32 us
-//     for the ~35 blocks that have rows, 42 us with all 64 (6.4 TB/s).
+//     32768 x 4096 x 2048 in 16 uneven groups 571 us = 963 TFLOP/s (542 to 579 over machines and group sizes; 128 x 128 tiles 620), the gradients of
+//     16384 x 2048 x 1536 in 16 groups 270 us, 244 if the groups are even.
+//   * a few rows a group: the weights, each read once.  16 x 64 tiles, every wave a quarter of a stage's sum: 64 rows of 2048 x 1024 blocks 27 to 34 us
+//     for the 30 to 40 blocks that have rows, 40 us with all 64 (6.7 TB/s).
 //   * in between: bytes from L2 to LDS (about 9.5 TB/s) and the latency of a stage; what helped was more workgroups on a CU, so two stages rather than three
 //     or four wherever the tiles fill the CUs (8192 x 1024 x 1024 fp32, 64 x 64 tiles: 144 us with two, 152 with three, 161 with four), and deep or wide
 //     stages where they do not (40 x 2048 x 2048 fp16: 12.3 -> 6.5 us with 8 waves sharing a 256-deep stage).
-//   * fp32 goes through the exact fp32 matrix instruction: 8192 x 1024 x 1024 at 131 TFLOP/s with 128 x 128 tiles.
-//   * 12013 x 61 x 512 fp32 (20 us; its stores alone take 6.3, its products 5.6, its loads 5.4): the three hardly overlap, since the workgroups of a CU
-//     start together; runs of column tiles, other tiles and deeper stages left it at 20 to 22 us.
-//   * odd strides (16 bit): a direct load wants 4-byte addresses; through registers 3001 x 777 x 1111 fp16 takes 18.3 us, 776 x 1112 14.8 directly.
+//   * fp32 goes through the exact fp32 matrix instruction: 8192 x 1024 x 1024 at 132 TFLOP/s with 128 x 128 tiles.
+//   * 12013 x 61 x 512 fp32 (20 us; with all but its stores, its products or its loads taken out of a copy of the kernel 6.3, 5.6, 5.4): the three hardly
+//     overlap, since the workgroups of a CU start together; runs of column tiles, other tiles and deeper stages left it at 20 to 22 us.
+//   * odd strides (16 bit): a direct load wants 4-byte addresses; through registers 3001 x 777 x 1111 fp16 takes 19.5 us, 776 x 1112 14.7 directly.
+//   * many groups: every workgroup looks its group up, 64 at a time, and every group may add a row tile.  65536 x 64 x 64 bf16 takes 10 us in 64 groups, 23 in
+//     1024, 379 in 8192 and 18.7 ms in 65536 of one row each: the look-up is all of it from a thousand groups on.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -94,6 +97,8 @@ template <typename S> struct Piece { static constexpr int V = 16 / sizeof(S); S 
 //   CC (contraction contiguous)   row = e; piece p stands at p ^ (e & 7), so 8 lanes that read one piece of 8 rows meet different banks
 //   !CC                           row = c; 16 bit: 32-byte blocks, block b stands at b ^ swz(c): the 8 rows c .. c + 3, c + 8 .. c + 11 that half a
 //                                 wave's transposed read touches meet different banks; fp32: 64-byte blocks, b ^ (c >> 2 & 3), for rows 4 lk + j
+// Short rows have too few places for that: fp32 of 32 values two for four rows (19 % of the LDS cycles of the 32 x 32 product tiles are conflicts, 20 % in the
+// 32 x 64 gradient tiles), 16 bit of 64 values four for eight (12 % in the 16 x 64 tiles); the 128 and 256 wide ones have none.
 template <typename S, bool CC, int E, int BK>
 struct Tile {
     static constexpr bool H = sizeof(S) == 2;
@@ -783,7 +788,7 @@ template <int BK> using AnyK = Shape<32, 32, BK, 1, 1, 8, 2, EDGE>;
 
 // Which tile, by the rows a group has on average, the widths, and how many tiles that makes for 256 CUs.  Large tiles fetch each value less often, small
 // ones fill the card.  us, the chosen shape and the next best:
-//   16 bit   T256    32768 x 4096 x 2048, 16 groups   617 : 656 (128 x 128)        T128     8000 x 1024 x 1024, 8 groups    24.7 : 32.3 (128 x 64)
+//   16 bit   T256    32768 x 4096 x 2048, 16 groups   572 : 620 (128 x 128)        T128     8000 x 1024 x 1024, 8 groups    24.7 : 32.3 (128 x 64)
 //            T128run 30000 x 64 x 1024, 10 groups    25.2 : 30.1 (T128)            T128deep 3001 x 1112 x 776, 7 groups     19.6 : 20.9 (128 x 64)
 //            T64deep 500 x 2048 x 2048, 8 groups     15.5 : 20.8 (T64), 25.4 (T128) T64      8000 x 1024 x 1024, 8 groups    36.4 : 40.8 (T64deep)
 //            T32     1000 x 512 x 512, 4 groups       5.5 : 6.2 (T64)              T32k     100 x 3000 x 300, 4 groups       8.4 : 11.8 (T32)
@@ -832,8 +837,9 @@ int product_pick(const ProductP& p, hipStream_t st) {
     if (k >= 512 && tiles(r, p.N, 32, 32) < 2 * kCus) return launch<TT, WT, AnyK<1024 / (int)sizeof(typename TT::S)>>(p, st);
     return launch<TT, WT, Any>(p, st);
 }
-// Few tiles with long sums: rows a part (0: the sums stay whole).  61 x 512 weights in 2 groups from 1024 rows each are 16 tiles of 64 x 64: 8.7 us in
-// parts.  From 64 tiles on whole sums are faster: 512 x 512 in 2 groups from 1024 rows each (128 tiles), both gradients, 27.5 us whole, 35.3 in parts.
+// Few tiles with long sums: rows a part (0: the sums stay whole).  us of the kernels in parts and whole (a call on its own pays 6 us more on the host for the
+// second launch and the workspace): 61 x 512 weights from 2048 rows in one group 8.9 : 16.1, from 20000 26 : 147; 512 x 1 from 1024 10.4 : 38.9; 61 x 512 from
+// 600 8.0 : 6.9.  From 64 tiles on whole sums are faster: 512 x 512 in 2 groups from 1024 rows each (128 tiles), both gradients, 27.5 whole, 35.3 in parts.
 int part_rows(int rows, int K, int N, int G) {
     const int64_t blocks = G * tiles(K, N, 64, 64), mean = rows / G;
     if (blocks >= 64 || mean < 512) return 0;

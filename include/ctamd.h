@@ -313,6 +313,7 @@ int ct_trim_mean(const double* stack, int k, int n3, double cut, double* out, ct
  * Rows behind offsets[G]: zero with fill_tail, else left as they were.  y must not overlap an operand.  Sums are 32-bit, fp32
  * products exact; their order depends on the sizes and on the alignment and layout of x and w, never on values or timing.  fp32 sums are folded every
  * 512 to 2048 steps of a wave; those of 16-bit operands are single chains (of n values of one sign at most n 2^-24 off).
+ * Every tile looks its group up among all of them: fine for a thousand groups, slow for many thousands (65536 x 64 x 64: 23 us and 18.7 ms).
  * CT_ESHAPE: a row stride above 2^22 values, a width above 2^30, more than 2^16 groups, or more than 2^22 tiles (of at least 16 x 32 values). */
 int ct_grouped_product(int type, int out_type, const void* x, int64_t ldx, int rows, int K, const void* w, int64_t w_group_stride, int64_t ldw,
                        int w_transposed, int N, const int32_t* offsets, int G, const float* scale, const float* shift, int64_t affine_stride,
