@@ -64,3 +64,36 @@ def test_steps_in_a_row(clip):
     for i in (1, 2):
         for s in ("mean", "var"):
             assert np.abs(after[f"bn{i}"][s] - moving[f"{s}{i}"]).max() <= 2 * TOL * np.abs(moving[f"{s}{i}"]).max()
+
+
+def test_predictions_beside_training():
+    """Every prediction that another thread makes meanwhile is that of the weights before or after some step, and of none in between"""
+    import threading
+    import torch
+    x, _ = _batch(2000, 3)
+    model = ffn_mod.FFN().set_weights_dict(synth.make_ffn_weights(seed=6, gain=6.0))
+    model.compile(learning_rate=0.05, epsilon=1e-3, global_clipnorm=1.0)
+    seen, errors, done = [], [], threading.Event()
+
+    def predict():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not done.is_set():
+                    seen.append(model.predict(x))
+        except Exception as e:                             # reported below: a thread's exception is not the test's
+            errors.append(e)
+    versions = [model._training.weights()]
+    thread = threading.Thread(target=predict)
+    thread.start()
+    try:
+        for i in range(25):
+            model.train_on_batch(*_batch(128, i))
+            versions.append(model._training.weights())
+    finally:
+        done.set()
+        thread.join(60)
+    assert not thread.is_alive() and not errors and len(seen) > 1
+    allowed = [ffn_mod.FFN().set_weights_dict(w).predict(x) for w in versions]
+    which = [next((i for i, a in enumerate(allowed) if np.array_equal(a, s)), None) for s in seen]
+    assert None not in which and which == sorted(which)
+    assert np.array_equal(model.predict(x), allowed[-1]) and not np.array_equal(allowed[0], allowed[-1])
