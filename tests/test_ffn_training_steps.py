@@ -89,6 +89,10 @@ def test_predictions_beside_training():
         for i in range(25):
             model.train_on_batch(*_batch(128, i))
             versions.append(model._training.weights())
+        for _ in range(1000):                              # (a slow start of the thread is no failure)
+            if len(seen) > 1 or errors:
+                break
+            done.wait(0.01)
     finally:
         done.set()
         thread.join(60)
